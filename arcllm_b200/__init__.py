@@ -12,14 +12,16 @@ import threading
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libarcllm_cuda.so")
 
-GGML_F32, GGML_F16, GGML_Q4_K, GGML_Q6_K = 0, 1, 12, 14
+GGML_F32, GGML_F16, GGML_Q4_K, GGML_Q6_K, GGML_BF16 = 0, 1, 12, 14, 30
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+ROPE_INTERLEAVED, ROPE_HALVES = 0, 1
 TYPE_EXEC148 = 148  # EXEC148 image of a Q4_K matrix (route B of the Q4 FFN-down capability)
 Q4K_BLOCK_BYTES, Q6K_BLOCK_BYTES = 144, 210
 
 _lock = threading.Lock()
 _lib = None
 
-_vp, _u32, _u64, _f32, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_float, C.c_int
+_vp, _u32, _u64, _f32, _i32, _f64 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_float, C.c_int, C.c_double
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 SIGNATURES = {
@@ -67,6 +69,15 @@ SIGNATURES = {
     "arcllm_cuda_attention_decode_noalloc": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp],
     "arcllm_cuda_embed": [_i32, _vp, _vp, _u32, _u32, _vp, _vp],
     "arcllm_cuda_argmax": [_vp, _u32, _vp, C.POINTER(_u32), C.POINTER(_i32), _vp],
+    "arcllm_cuda_paged_plan": [_vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "arcllm_cuda_rope_freqs": [_i32, _u32, _f64, _f64, _f64, _vp, _vp],
+    "arcllm_cuda_rope_kv_paged": [_i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _u32, _i32, _f32, _vp,
+                                  _vp, _u32, _u32, _vp, _vp, _u64, _vp],
+    "arcllm_cuda_attention_paged_workspace": [_u32, _u32, _u32, C.POINTER(_u64)],
+    "arcllm_cuda_attention_paged": [_vp, _u64, _vp, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _f32, _u32, _u32,
+                                    _vp, _u64, _vp, _u64, _vp],
+    "arcllm_cuda_logits_process": [_i32, _vp, _u64, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                   _vp, _u32, _vp, _u64, _vp, _vp],
     "arcllm_cuda_set_launch_overlap": [_i32],
     "arcllm_cuda_set_device": [_i32],
     "arcllm_cuda_device_count": [C.POINTER(C.c_int)],
@@ -156,6 +167,12 @@ class Layer(C.Structure):
                 ("wk", _vp), ("bk", _vp), ("type_k", _i32), ("wv", _vp), ("bv", _vp), ("type_v", _i32),
                 ("wo", _vp), ("type_o", _i32), ("ffn_norm", _vp), ("w_gate", _vp), ("w_up", _vp),
                 ("type_gate_up", _i32), ("w_down", _vp), ("type_down", _i32)]
+
+
+class PagedKV(C.Structure):
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("page_stride", _u64), ("token_stride", _u32),
+                ("head_stride", _u32), ("n_pages", _u32), ("page_size", _u32), ("kv_heads", _u32),
+                ("head_dim", _u32), ("type", _i32)]
 
 
 class GenStats(C.Structure):

@@ -1,0 +1,582 @@
+// Attention of a batch's new rows over a paged KV cache (B200, sm_100a).
+//
+// o_i = sum_j softmax_j(scale q_i . k_j) v_j over the positions j that row i
+// sees: j <= p_i, and with a window j > p_i - window or j < sinks.  The query
+// heads of one KV head share its keys and values, so (row, head of the group)
+// pairs are packed into the rows of one matrix operand.  Work is counted in
+// units (an item's tile of positions), the units of all requests stand in one
+// line, and every CTA takes an equal stretch of it: contexts of any mixture of
+// lengths keep all SMs equally busy.  What is split between CTAs is joined by
+// a second, small launch.
+#include <algorithm>
+#include <cmath>
+
+#include "arcllm_cuda_internal.h"
+#include "attention_paged.cuh"
+#include "decode_ops.h"
+
+namespace arc {
+namespace {
+
+using namespace paged;
+
+// ---- few rows: one warp per stretch ------------------------------------------
+constexpr uint32_t kRowWarps = 8, kRowTile = 16, kRowMax = 16;  // packed rows of an item
+
+struct Segment {  // an unfinished item of a warp
+    uint32_t valid, u0, u1, r, kvh, mt;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// Query rows of an item: as many as fit kRowMax packed rows.
+__host__ __device__ __forceinline__ uint32_t rows_per_item(uint32_t gq) { return kRowMax / gq; }
+
+// Position in the line of units: request, KV head, row group, tile.
+struct Cursor {
+    uint32_t r, kvh, mt, i, mts, nt;
+    Req q;
+    Span s;
+    __device__ __forceinline__ void enter(const Args& a) {  // request r's sizes
+        bool bad = false;
+        load_req(a, r, q, bad);
+        const uint32_t rpi = rows_per_item(a.gq);
+        mts = (q.n + rpi - 1u) / rpi;
+        s = span_of<kRowTile>(a, q.p0, q.p0 + q.n - 1u);
+        nt = s.n;
+    }
+    __device__ __forceinline__ void seek(const Args& a, const uint32_t* off, uint32_t u) {
+        uint32_t lo = 0, hi = a.n_requests;
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (off[mid] <= u)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        r = lo;
+        enter(a);
+        uint32_t rem = u - off[r];
+        i = rem % nt;
+        rem /= nt;
+        mt = rem % mts;
+        kvh = rem / mts;
+    }
+    __device__ __forceinline__ void next(const Args& a, const uint32_t* off) {
+        if (++i < nt) return;
+        i = 0;
+        if (++mt < mts) return;
+        mt = 0;
+        if (++kvh < a.kv_heads) return;
+        kvh = 0;
+        const uint32_t end = off[r + 1];
+        do ++r;
+        while (r < a.n_requests && off[r + 1] == end);  // requests without units
+        if (r < a.n_requests) enter(a);
+    }
+};
+
+// Units of every request before request r, in off[0 .. n]; all threads of the
+// CTA.  Returns the total, or 0 where it does not fit 31 bits.
+template <typename Units>
+__device__ __forceinline__ uint32_t scan_units(const Args& a, uint32_t* off, unsigned int* err, Units units) {
+    __shared__ unsigned long long s_warp[32];
+    __shared__ int s_bad;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (threadIdx.x == 0) s_bad = 0, off[0] = 0;
+    unsigned long long base = 0;
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += blockDim.x) {
+        const uint32_t r = r0 + threadIdx.x;
+        bool bad = false;
+        unsigned long long v = 0;
+        if (r < a.n_requests) v = units(r, bad);
+        __syncthreads();
+        if (bad) s_bad = 1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= (uint32_t)o) v += x;
+        }
+        if (lane == 31u) s_warp[warp] = v;
+        __syncthreads();
+        unsigned long long all = 0;
+        for (uint32_t w = 0; w < warps; ++w) {
+            if (w < warp) v += s_warp[w];
+            all += s_warp[w];
+        }
+        if (r < a.n_requests) off[r + 1] = (uint32_t)(base + v);
+        base += all;
+    }
+    __syncthreads();
+    const bool too_many = base > 0x7fffffffull;
+    if (threadIdx.x == 0 && blockIdx.x == 0 && (s_bad || too_many)) raise_error(err, ARC_DEV_ERR_BOUNDS);
+    return too_many ? 0u : (uint32_t)base;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kRowWarps * 32, 1)
+    attn_paged_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a,
+                           uint32_t slot_rows, uint32_t stages, Record* __restrict__ recs, float* __restrict__ parts,
+                           unsigned int* err) {
+    constexpr uint32_t HB = kRowTile * 128u;           // one box: 16 positions x 64 dims
+    constexpr uint32_t NH = D / 64;                    // boxes per K or V tile
+    constexpr uint32_t TILE = NH * HB, STAGE = 2u * TILE;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
+    const uint32_t slot_floats = slot_rows * (D + 2u);
+    uint8_t* rings = smem;
+    float* firsts = reinterpret_cast<float*>(smem + kRowWarps * stages * STAGE);
+    uint32_t* off = reinterpret_cast<uint32_t*>(firsts + kRowWarps * slot_floats);
+    __shared__ uint64_t bars[kRowWarps][4];
+    __shared__ Segment segs[kRowWarps][2];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    if (lane < stages) mbar_init(&bars[warp][lane], 1);
+    if (lane < 2) segs[warp][lane].valid = 0;
+    fence_mbar_init();
+    pdl_trigger();
+    pdl_wait();  // lengths, queries and pages come from the preceding kernels
+    const uint32_t rpi = rows_per_item(a.gq);
+    const uint32_t total = scan_units(a, off, err, [&](uint32_t r, bool& bad) -> unsigned long long {
+        Req q;
+        if (!load_req(a, r, q, bad)) return 0;
+        return (unsigned long long)a.kv_heads * ((q.n + rpi - 1u) / rpi) *
+               span_of<kRowTile>(a, q.p0, q.p0 + q.n - 1u).n;
+    });
+    // equal shares of whole rounds of the CTA's warps
+    const uint32_t per = max(((total + gridDim.x - 1u) / gridDim.x + kRowWarps - 1u) / kRowWarps, 1u) * kRowWarps;
+    const uint32_t U0 = min(blockIdx.x * per, total), U1 = min(U0 + per, total);
+    if (tid == 0) recs[blockIdx.x].valid = 0;
+    if (U0 == U1) return;
+    const uint32_t pw = per / kRowWarps;
+    const uint32_t u0 = min(U0 + warp * pw, U1), n_units = min(u0 + pw, U1) - u0;
+
+    uint8_t* ring = rings + warp * stages * STAGE;
+    bool bad_page = false;
+    if (n_units) {
+        Cursor ci, cc;
+        ci.seek(a, off, u0);
+        cc = ci;
+        auto entry = [&](const Cursor& c) -> int {  // the page of a cursor's tile
+            return __ldg(a.table + (uint64_t)c.r * a.table_stride + c.s.tile(c.i) * kRowTile / a.page_size);
+        };
+        int page = entry(ci);
+        uint32_t issued = 0, si = 0;
+        auto issue = [&]() {
+            const uint32_t pos = ci.s.tile(ci.i) * kRowTile;
+            uint64_t* bar = &bars[warp][si];
+            uint8_t* st = ring + si * STAGE;
+            if ((uint32_t)page >= a.n_pages) {
+                bad_page = true;
+                page = (int)a.n_pages;  // reads zeros
+            }
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bar, STAGE);
+                const int tok = (int)(pos % a.page_size);
+#pragma unroll
+                for (uint32_t h = 0; h < NH; ++h) {
+                    tma_page(st + h * HB, &kmap, (int)(64u * h), tok, (int)ci.kvh, page, bar);
+                    tma_page(st + TILE + h * HB, &vmap, (int)(64u * h), tok, (int)ci.kvh, page, bar);
+                }
+            }
+            si = si + 1u == stages ? 0u : si + 1u;
+            ++issued;
+            if (issued < n_units) {
+                ci.next(a, off);
+                page = entry(ci);  // used one tile later
+            }
+        };
+        for (uint32_t s = 0; s < stages && s < n_units; ++s) issue();
+
+        uint32_t qa[D / 16][4];
+        float o[D / 8][4];
+        float m[2], l[2];
+        uint32_t pos_of[2];
+        uint32_t s_cons = 0, parity = 0, seg_u0 = u0;
+        uint32_t item_rows = 0, item_row0 = 0;
+        bool first_seg = true, ok = true;
+        uint32_t it = 0;
+        for (; it < n_units; ++it) {
+            if (it == 0 || cc.i == 0) {  // a new item: its queries into A fragments
+                seg_u0 = u0 + it;
+                first_seg = it == 0;
+                const uint32_t q0 = cc.mt * rpi;
+                item_rows = min(rpi, cc.q.n - q0) * a.gq;
+                item_row0 = cc.q.row0 + q0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t ri = min(g + 8u * h, item_rows - 1u), qr = ri / a.gq;
+                    pos_of[h] = cc.q.p0 + q0 + qr;
+                    const uint16_t* src = a.q + (uint64_t)(item_row0 + qr) * a.q_stride +
+                                          (cc.kvh * a.gq + ri - qr * a.gq) * D + 2u * t;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        qa[kk][h] = *reinterpret_cast<const uint32_t*>(src + 16 * kk);
+                        qa[kk][h + 2] = *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8);
+                    }
+                    m[h] = -INFINITY, l[h] = 0.f;
+                }
+#pragma unroll
+                for (int nt = 0; nt < D / 8; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
+            }
+            if (!mbar_wait(&bars[warp][s_cons], parity, err)) {
+                ok = false;
+                break;
+            }
+            const uint32_t ks = smem_addr(ring + s_cons * STAGE), vs = ks + TILE;
+            const uint32_t mi = lane >> 3, mr = lane & 7u;
+            const uint32_t p_tile = cc.s.tile(cc.i) * kRowTile;
+            float sc[2][4];
+#pragma unroll
+            for (int pb = 0; pb < 2; ++pb) {
+                sc[pb][0] = sc[pb][1] = sc[pb][2] = sc[pb][3] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk += 2) {
+                    uint32_t b[4];
+                    const uint32_t ch = 2u * (kk & 3) + mi;  // 16-byte column of the 128-byte row
+                    ldmatrix4(b, ks + (kk >> 2) * HB + (8u * pb + mr) * 128u + ((ch ^ mr) << 4));
+                    mma_16816<BF16>(sc[pb], qa[kk], b[0], b[1]);
+                    mma_16816<BF16>(sc[pb], qa[kk + 1], b[2], b[3]);
+                }
+            }
+            // positions that row g + 8(c >> 1) does not see
+#pragma unroll
+            for (int pb = 0; pb < 2; ++pb)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    sc[pb][c] = visible(a, pos_of[c >> 1], p_tile + 8u * pb + 2u * t + (c & 1)) ? sc[pb][c] * a.scale_log2
+                                                                                                 : -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[h], mx);
+                const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far: all weights 0
+                const float alpha = ex2(m[h] - ref);
+                m[h] = mn;
+                float ps = 0.f;
+#pragma unroll
+                for (int pb = 0; pb < 2; ++pb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        sc[pb][2 * h + c] = ex2(sc[pb][2 * h + c] - ref);
+                        ps += sc[pb][2 * h + c];
+                    }
+                l[h] = fmaf(l[h], alpha, ps);  // this lane's columns; the quad's are added at the end
+#pragma unroll
+                for (int nt = 0; nt < D / 8; ++nt) o[nt][2 * h] *= alpha, o[nt][2 * h + 1] *= alpha;
+            }
+            // Weights in the cache's type for the matrix product: half a step of it each, as the output's own rounding.
+            const uint32_t pa[4] = {pack16<BF16>(sc[0][0], sc[0][1]), pack16<BF16>(sc[0][2], sc[0][3]),
+                                    pack16<BF16>(sc[1][0], sc[1][1]), pack16<BF16>(sc[1][2], sc[1][3])};
+            // What no row of the item sees (behind the last position, before the window) may hold anything, and
+            // 0 * NaN would reach the sums: such values are read as zero.  A fragment register holds positions
+            // 8(j & 1) + 2t, + 1.
+            const uint32_t p_last = cc.q.p0 + cc.q.n - 1u;
+            const uint32_t p_from = a.window && cc.q.p0 >= a.window ? cc.q.p0 - a.window + 1u : 0u;
+            const bool edge = p_tile + kRowTile - 1u > p_last || (p_tile < p_from && p_tile + kRowTile > a.sinks) ;
+            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t p = p_tile + 8u * j + 2u * t;
+                    const bool k0 = p <= p_last && (p >= p_from || p < a.sinks);
+                    const bool k1 = p + 1u <= p_last && (p + 1u >= p_from || p + 1u < a.sinks);
+                    keep[j] = (k0 ? 0xffffu : 0u) | (k1 ? 0xffff0000u : 0u);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < D / 8; nt += 2) {
+                uint32_t v[4];
+                const uint32_t ch = (nt & 7) + (mi >> 1);
+                ldmatrix4_trans(v, vs + (nt >> 3) * HB + (8u * (mi & 1u) + mr) * 128u + ((ch ^ mr) << 4));
+                mma_16816<BF16>(o[nt], pa, v[0] & keep[0], v[1] & keep[1]);
+                mma_16816<BF16>(o[nt + 1], pa, v[2] & keep[0], v[3] & keep[1]);
+            }
+            __syncwarp();
+            s_cons = s_cons + 1u == stages ? 0u : s_cons + 1u;
+            if (s_cons == 0) parity ^= 1u;
+            const bool ends = cc.i + 1u == cc.nt;
+            if (issued < n_units) issue();
+            if (ends || it + 1u == n_units) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                }
+                const uint32_t item_u0 = u0 + it - cc.i;  // may lie before this warp's stretch
+                if (ends && seg_u0 == item_u0) {  // all of the item: its output
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t ri = g + 8u * h, qr = ri / a.gq;
+                        if (ri >= item_rows) continue;
+                        uint16_t* dst = a.out + (uint64_t)(item_row0 + qr) * a.out_stride +
+                                        (cc.kvh * a.gq + ri - qr * a.gq) * D + 2u * t;
+                        const float inv = 1.f / l[h];
+#pragma unroll
+                        for (int nt = 0; nt < D / 8; ++nt)
+                            *reinterpret_cast<uint32_t*>(dst + 8 * nt) =
+                                pack16<BF16>(o[nt][2 * h] * inv, o[nt][2 * h + 1] * inv);
+                    }
+                } else {  // a part: into shared memory (the last one over the ring, which nothing fills any more)
+                    float* slot = first_seg ? firsts + warp * slot_floats : reinterpret_cast<float*>(ring);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t ri = g + 8u * h;
+                        if (ri >= item_rows) continue;
+#pragma unroll
+                        for (int nt = 0; nt < D / 8; ++nt)
+                            *reinterpret_cast<float2*>(slot + ri * D + 8 * nt + 2u * t) =
+                                make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
+                        if (t == 0)
+                            *reinterpret_cast<float2*>(slot + slot_rows * D + 2u * ri) = make_float2(m[h], l[h]);
+                    }
+                    if (lane == 0) segs[warp][first_seg ? 0 : 1] = {1u, item_u0, item_u0 + cc.nt, cc.r, cc.kvh, cc.mt};
+                }
+            }
+            if (it + 1u < n_units) cc.next(a, off);
+        }
+        if (!ok) {  // a copy did not arrive: wait (bounded) for the others before the CTA may end
+            for (uint32_t k = it + 1u; k < issued; ++k) {
+                s_cons = s_cons + 1u == stages ? 0u : s_cons + 1u;
+                if (s_cons == 0) parity ^= 1u;
+                mbar_wait(&bars[warp][s_cons], parity, err);
+            }
+        }
+        if (bad_page && lane == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
+    }
+    __syncthreads();
+    // Runs of parts of one item, warp by warp; an item that lies within this CTA's stretch is done here.
+    for (uint32_t k = 0; k < 2u * kRowWarps;) {
+        const Segment sg = segs[k >> 1][k & 1u];
+        if (!sg.valid) {
+            ++k;
+            continue;
+        }
+        uint32_t e = k + 1u;
+        while (e < 2u * kRowWarps && (!segs[e >> 1][e & 1u].valid || segs[e >> 1][e & 1u].u0 == sg.u0)) ++e;
+        Req q;
+        bool bad = false;
+        load_req(a, sg.r, q, bad);
+        const uint32_t q0 = sg.mt * rpi, rows = min(rpi, q.n - q0) * a.gq;
+        const bool whole = sg.u0 >= U0 && sg.u1 <= U1;
+        const uint32_t slot_no = sg.u0 < U0 ? 0u : 1u;
+        float* part = parts + (uint64_t)(blockIdx.x * 2u + slot_no) * (kRowMax * (D + 2u));
+        if (!whole && slot_no == 1u && tid == 0)
+            recs[blockIdx.x] = {1u, (sg.u1 - 1u) / per, q.row0 + q0, rows, sg.kvh, {0, 0, 0}};
+        for (uint32_t x = tid; x < rows * (D / 4u); x += kRowWarps * 32u) {
+            const uint32_t ri = x / (D / 4u), c = (x - ri * (D / 4u)) * 4u;
+            float M = -INFINITY;
+            for (uint32_t j = k; j < e; ++j)
+                if (segs[j >> 1][j & 1u].valid) {
+                    const float* slot = (j & 1u) ? reinterpret_cast<const float*>(rings + (j >> 1) * stages * STAGE)
+                                                 : firsts + (j >> 1) * slot_floats;
+                    M = fmaxf(M, slot[slot_rows * D + 2u * ri]);
+                }
+            const float ref = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t j = k; j < e; ++j)
+                if (segs[j >> 1][j & 1u].valid) {
+                    const float* slot = (j & 1u) ? reinterpret_cast<const float*>(rings + (j >> 1) * stages * STAGE)
+                                                 : firsts + (j >> 1) * slot_floats;
+                    const float2 ml = *reinterpret_cast<const float2*>(slot + slot_rows * D + 2u * ri);
+                    const float4 v = *reinterpret_cast<const float4*>(slot + ri * D + c);
+                    const float f = ex2(ml.x - ref);
+                    L = fmaf(ml.y, f, L);
+                    A.x = fmaf(v.x, f, A.x), A.y = fmaf(v.y, f, A.y);
+                    A.z = fmaf(v.z, f, A.z), A.w = fmaf(v.w, f, A.w);
+                }
+            if (whole) {
+                const uint32_t qr = ri / a.gq;
+                const float inv = 1.f / L;
+                *reinterpret_cast<uint2*>(a.out + (uint64_t)(q.row0 + q0 + qr) * a.out_stride +
+                                          (sg.kvh * a.gq + ri - qr * a.gq) * D + c) =
+                    make_uint2(pack16<BF16>(A.x * inv, A.y * inv), pack16<BF16>(A.z * inv, A.w * inv));
+            } else {
+                *reinterpret_cast<float4*>(part + ri * D + c) = A;
+                if (c == 0) *reinterpret_cast<float2*>(part + kRowMax * D + 2u * ri) = make_float2(M, L);
+            }
+        }
+        k = e;
+    }
+}
+
+// ---- join ---------------------------------------------------------------------
+// Block (c, part): the item that CTA c began and later CTAs went on with.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Record* __restrict__ recs,
+                                                              const float* __restrict__ parts, uint32_t max_rows) {
+    pdl_trigger();
+    pdl_wait();
+    const Record rc = recs[blockIdx.x];
+    if (!rc.valid) return;
+    const uint32_t stride = max_rows * (D + 2u);
+    for (uint32_t x = blockIdx.y * blockDim.x + threadIdx.x; x < rc.rows * (D / 4u); x += gridDim.y * blockDim.x) {
+        const uint32_t ri = x / (D / 4u), c = (x - ri * (D / 4u)) * 4u;
+        constexpr uint32_t CH = 8;  // parts whose loads are in flight together
+        float M = -INFINITY, L = 0.f;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t j0 = blockIdx.x; j0 <= rc.last_cta; j0 += CH) {
+            float2 ml[CH];
+            float4 v[CH];
+#pragma unroll
+            for (uint32_t j = 0; j < CH; ++j) {
+                ml[j] = make_float2(-INFINITY, 0.f);
+                v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (j0 + j <= rc.last_cta) {
+                    const float* p = parts + (uint64_t)((j0 + j) * 2u + (j0 + j == blockIdx.x ? 1u : 0u)) * stride;
+                    ml[j] = *reinterpret_cast<const float2*>(p + max_rows * D + 2u * ri);
+                    v[j] = *reinterpret_cast<const float4*>(p + ri * D + c);
+                }
+            }
+            float mn = M;
+#pragma unroll
+            for (uint32_t j = 0; j < CH; ++j) mn = fmaxf(mn, ml[j].x);
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float f0 = ex2(M - ref);
+            L *= f0, A.x *= f0, A.y *= f0, A.z *= f0, A.w *= f0;
+#pragma unroll
+            for (uint32_t j = 0; j < CH; ++j) {
+                const float f = ex2(ml[j].x - ref);
+                L = fmaf(ml[j].y, f, L);
+                A.x = fmaf(v[j].x, f, A.x), A.y = fmaf(v[j].y, f, A.y);
+                A.z = fmaf(v[j].z, f, A.z), A.w = fmaf(v[j].w, f, A.w);
+            }
+            M = mn;
+        }
+        const uint32_t qr = ri / a.gq;
+        const float inv = 1.f / L;
+        *reinterpret_cast<uint2*>(a.out + (uint64_t)(rc.row0 + qr) * a.out_stride +
+                                  (rc.kvh * a.gq + ri - qr * a.gq) * D + c) =
+            make_uint2(pack16<BF16>(A.x * inv, A.y * inv), pack16<BF16>(A.z * inv, A.w * inv));
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+struct Workspace {
+    Record* recs;
+    float* parts;
+};
+constexpr uint64_t kRecBytes = (sizeof(Record) * kSms + 255u) / 256u * 256u;
+uint64_t rows_part_bytes(uint32_t d) { return 4ull * kSms * 2u * kRowMax * (d + 2u); }
+
+// Tensor map of K or V: boxes of `tokens` positions x 64 dims of one head of one page, 128-byte swizzle.
+int encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return set_error(ARC_E_CUDA, "attention paged: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {kv.head_dim, kv.page_size, kv.kv_heads, kv.n_pages};
+    const cuuint64_t strides[3] = {2ull * kv.token_stride, 2ull * kv.head_stride, 2ull * kv.page_stride};
+    const cuuint32_t box[4] = {64, tokens, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult rc =
+        fn(map, kv.type == ARC_GGML_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+           const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? ARC_OK : set_error(ARC_E_CUDA, "attention paged: tensor map of the pages");
+}
+
+template <int D, bool BF16>
+int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args& a, cudaStream_t stream) {
+    constexpr uint32_t kStage = 4u * kRowTile * D, kMost = 232448u - 2048u;  // 227 KB less the static arrays
+    CUtensorMap kmap, vmap;
+    int st = encode_pages(&kmap, kv, kv.k_pages, kRowTile);
+    if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, kRowTile);
+    if (st != ARC_OK) return st;
+    uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+    Record* recs = reinterpret_cast<Record*>(ws);
+    float* parts = reinterpret_cast<float*>(ws + kRecBytes);
+    const uint32_t rpi = rows_per_item(a.gq);
+    const uint32_t slot_rows = std::min(rpi, a.max_new) * a.gq <= 8u ? 8u : 16u;
+    const uint32_t fixed = 1024u + kRowWarps * slot_rows * (D + 2u) * 4u + 4u * (a.n_requests + 1u);
+    const uint32_t stages = std::min(4u, (kMost - fixed) / (kRowWarps * kStage));
+    const uint32_t smem = fixed + kRowWarps * stages * kStage;
+    cudaError_t e = cudaFuncSetAttribute(attn_paged_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)kMost);
+    if (e == cudaSuccess)
+        e = launch_kernel(attn_paged_rows_kernel<D, BF16>, dim3(kSms), dim3(kRowWarps * 32u), smem, stream, kmap, vmap,
+                          a, slot_rows, stages, recs, parts, dev_error_word());
+    if (e == cudaSuccess)
+        e = launch_kernel(attn_paged_join_kernel<D, BF16>, dim3(kSms, 2), dim3(256), 0, stream, a, recs, parts,
+                          kRowMax);
+    return launch_checked(e, "attention paged launch");
+}
+
+}  // namespace
+
+int attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint64_t* out) {
+    if (!out) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged workspace: null out");
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads)
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged workspace: q_heads % kv_heads");
+    if (head_dim != 64u && head_dim != 128u)
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged workspace: head_dim must be 64 or 128");
+    *out = kRecBytes + rows_part_bytes(head_dim);
+    return ARC_OK;
+}
+
+int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStream_t stream) {
+    if (p.n_requests == 0 || p.max_rows == 0 || p.max_new == 0) return ARC_OK;
+    if (!p.q || !p.block_table || !p.row_start || !p.kv_total || !p.out || !p.workspace)
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: null pointer");
+    uint64_t need = 0;
+    const int st = attention_paged_workspace(p.q_heads, kv.kv_heads, kv.head_dim, &need);
+    if (st != ARC_OK) return st;
+    const uint32_t gq = p.q_heads / kv.kv_heads;
+    if (gq > 16u) return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 16 query heads per KV head");
+    if (kv.page_size % 16u) return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: page_size must be a multiple of 16");
+    if (p.n_requests > kMaxRequests)
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 4096 requests");
+    if (p.max_rows > 0x7fffffffu || p.table_stride == 0)
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: bad shape");
+    if (!(p.scale > 0.f) || !std::isfinite(p.scale))
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: scale must be positive");
+    const uint64_t width = (uint64_t)p.q_heads * kv.head_dim;
+    if (p.q_stride < width || p.out_stride < width)
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: a row stride shorter than the row");
+    auto off16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) != 0u; };
+    if (off16(p.q) || off16(p.out) || off16(kv.k_pages) || off16(kv.v_pages) || off16(p.workspace) ||
+        p.q_stride % 8u || p.out_stride % 8u || kv.page_stride % 8u || kv.token_stride % 8u || kv.head_stride % 8u)
+        return set_error(ARC_E_ALIGNMENT, "attention paged: pointers and strides of 16 bytes");
+    if (kv.page_stride >= (1ull << 39) )
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: page stride past 2^40 bytes");
+    if (p.workspace_bytes < need) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: workspace too small");
+    Args a{};
+    a.q = static_cast<const uint16_t*>(p.q);
+    a.out = static_cast<uint16_t*>(p.out);
+    a.q_stride = p.q_stride, a.out_stride = p.out_stride;
+    a.table = p.block_table, a.table_stride = p.table_stride;
+    a.row_start = p.row_start, a.kv_total = p.kv_total;
+    a.n_requests = p.n_requests, a.max_rows = p.max_rows, a.max_new = p.max_new;
+    a.kv_heads = kv.kv_heads, a.gq = gq, a.page_size = kv.page_size, a.n_pages = kv.n_pages;
+    a.scale_log2 = (float)((double)p.scale * 1.4426950408889634074);
+    a.window = p.window, a.sinks = p.window ? p.sinks : 0u;
+    const bool bf = kv.type == ARC_GGML_BF16;
+    if (kv.head_dim == 128u)
+        return bf ? launch_paged<128, true>(p, kv, a, stream) : launch_paged<128, false>(p, kv, a, stream);
+    return bf ? launch_paged<64, true>(p, kv, a, stream) : launch_paged<64, false>(p, kv, a, stream);
+}
+
+}  // namespace arc

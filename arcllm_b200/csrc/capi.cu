@@ -10,6 +10,7 @@
 #include "arcllm_cuda_internal.h"
 #include "common.cuh"
 #include "decode_ops.h"
+#include "paged_ops.h"
 #include "prefill_ops.h"
 
 namespace arc {
@@ -545,6 +546,74 @@ int arcllm_cuda_argmax(const float* logits, uint32_t n, void* scratch_dev, uint3
     *index_host = hk[0] ? ~(uint32_t)(hk[0] & 0xffffffffull) : 0u;
     if (finite_host) *finite_host = (nonfinite == 0 && hk[0] != 0) ? 1 : 0;
     return ARC_OK;
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_paged_plan(const int32_t* kv_len, const int32_t* new_len, uint32_t n_requests, uint32_t page_size,
+                           uint32_t n_pages, const int32_t* free_pages, const int32_t* n_free, int32_t* block_table,
+                           uint32_t table_stride, uint32_t max_rows, int32_t* row_start, int32_t* kv_total,
+                           int32_t* positions, int32_t* slots, int32_t* n_free_out, void* stream) {
+    ARC_GUARD_BEGIN
+    return arc::paged_plan({kv_len, new_len, n_requests, page_size, n_pages, free_pages, n_free, block_table,
+                            table_stride, max_rows, row_start, kv_total, positions, slots, n_free_out},
+                           static_cast<cudaStream_t>(stream));
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_rope_freqs(int scaling, uint32_t rot_dim, double theta, double factor, double trained_ctx,
+                           double* freqs_host, float* attn_scale_host) {
+    ARC_GUARD_BEGIN
+    return arc::rope_freqs(scaling, rot_dim, theta, factor, trained_ctx, freqs_host, attn_scale_host);
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_rope_kv_paged(int act_type, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride,
+                              const void* v, uint64_t v_stride, const float* bq, const float* bk, const float* bv,
+                              const double* freqs, uint32_t rot_dim, int layout, float attn_scale,
+                              const int32_t* positions, const int32_t* slots, uint32_t rows, uint32_t q_heads,
+                              const arcllm_cuda_paged_kv* kv, void* q_out, uint64_t q_out_stride, void* stream) {
+    ARC_GUARD_BEGIN
+    const int st = arc::check_paged_kv(kv, "rope paged");
+    if (st != ARC_OK) return st;
+    return arc::rope_kv_paged(act_type,
+                              {q, k, v, q_stride, k_stride, v_stride, q_out_stride, bq, bk, bv, freqs, rot_dim, layout,
+                               attn_scale, positions, slots, rows, q_heads, q_out},
+                              *kv, static_cast<cudaStream_t>(stream));
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint64_t* out) {
+    ARC_GUARD_BEGIN
+    return arc::attention_paged_workspace(q_heads, kv_heads, head_dim, out);
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_attention_paged(const void* q, uint64_t q_stride, const arcllm_cuda_paged_kv* kv,
+                                const int32_t* block_table, uint32_t table_stride, const int32_t* row_start,
+                                const int32_t* kv_total, uint32_t n_requests, uint32_t max_rows, uint32_t max_new,
+                                uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void* out,
+                                uint64_t out_stride, void* workspace, uint64_t workspace_bytes, void* stream) {
+    ARC_GUARD_BEGIN
+    const int st = arc::check_paged_kv(kv, "attention paged");
+    if (st != ARC_OK) return st;
+    return arc::attention_paged({q, q_stride, out_stride, block_table, table_stride, row_start, kv_total, n_requests,
+                                 max_rows, max_new, q_heads, scale, window, sinks, out, workspace, workspace_bytes},
+                                *kv, static_cast<cudaStream_t>(stream));
+    ARC_GUARD_END
+}
+
+int arcllm_cuda_logits_process(int type, const void* logits, uint64_t stride, uint32_t n_rows, uint32_t vocab,
+                               const int32_t* history, uint32_t history_stride, const int32_t* prompt_len,
+                               const int32_t* total_len, const float* repetition, const float* frequency,
+                               const float* presence, const int32_t* bias_start, const int32_t* bias_ids,
+                               const float* bias_values, const uint32_t* mask, uint32_t mask_stride, void* out,
+                               uint64_t out_stride, int32_t* best, void* stream) {
+    ARC_GUARD_BEGIN
+    return arc::logits_process(type,
+                               {logits, stride, out_stride, n_rows, vocab, history, history_stride, prompt_len,
+                                total_len, repetition, frequency, presence, bias_start, bias_ids, bias_values, mask,
+                                mask_stride, out, best},
+                               static_cast<cudaStream_t>(stream));
     ARC_GUARD_END
 }
 

@@ -53,7 +53,13 @@ enum arcllm_cuda_status {
     ARC_E_NCCL = 8
 };
 
-enum arcllm_ggml_type { ARC_GGML_F32 = 0, ARC_GGML_F16 = 1, ARC_GGML_Q4_K = 12, ARC_GGML_Q6_K = 14 };
+enum arcllm_ggml_type {
+    ARC_GGML_F32 = 0,
+    ARC_GGML_F16 = 1,
+    ARC_GGML_Q4_K = 12,
+    ARC_GGML_Q6_K = 14,
+    ARC_GGML_BF16 = 30 /* paged cache, its activations, batched logits */
+};
 /* Not a GGUF type: the EXEC148 image of a Q4_K matrix (primitive B of the
  * Q4 FFN-down capability, src/q4_down_exec148_materializer.h:14), 148 bytes
  * per super-block.  Accepted by arcllm_cuda_matvec (without gamma or bias)
@@ -378,6 +384,144 @@ ARCLLM_CUDA_API int arcllm_cuda_embed(int type, const void *table, const uint32_
  * `scratch_dev` holds 16 bytes. */
 ARCLLM_CUDA_API int arcllm_cuda_argmax(const float *logits, uint32_t n, void *scratch_dev, uint32_t *index_host,
                                        int *finite_host, void *stream);
+
+/* ---- a batch of requests over a paged KV cache -----------------------------
+ * Not in the reference (it serves one request from a contiguous cache,
+ * src/arcllm_v1_runtime.cpp:254-263): the step of a server that runs many
+ * requests at once.  arcllm_cuda_paged_plan lays the step out on the device,
+ * arcllm_cuda_rope_kv_paged and arcllm_cuda_attention_paged run per layer,
+ * arcllm_cuda_logits_process follows the LM head.  Nothing here allocates,
+ * synchronises or reads back: lengths stay on the device and a captured step
+ * replays with new ones.  Index arrays are int32.  Lengths or page numbers
+ * that no step can have set the device error word's bounds bit (bit 1). */
+
+/* One layer's cache.  Element (page, token, head, dim) of K and of V lies at
+ * page * page_stride + token * token_stride + head * head_stride + dim
+ * (elements), so pages may be stored token by token or head by head. */
+typedef struct {
+    void *k_pages, *v_pages;
+    uint64_t page_stride;
+    uint32_t token_stride, head_stride;
+    uint32_t n_pages, page_size, kv_heads, head_dim;
+    int type; /* ARC_GGML_F16 or ARC_GGML_BF16 */
+} arcllm_cuda_paged_kv;
+
+/* Lays out one step: request r (r < n_requests <= 8192) has kv_len[r] tokens
+ * in the cache and brings new_len[r] >= 0 new ones.  Writes
+ *   row_start[n_requests + 1]  first row of each request, and the row count;
+ *   kv_total[n_requests]       kv_len + new_len;
+ *   block_table                [n_requests][table_stride] page numbers; the
+ *                              entries that the new tokens need are filled with
+ *                              pages from the END of free_pages[0, *n_free), in
+ *                              request order, the others are left alone;
+ *   positions, slots[max_rows] of each new row: its place in its request, and
+ *                              page * page_size + token, its place in the cache;
+ *                              rows behind the last one get 0 and -1;
+ *   n_free_out                 how many free pages are left.
+ * A step that does not fit (more than max_rows rows, more pages than are free,
+ * a table row too short, a negative length) sets the bounds bit and lays out
+ * an empty step instead: row_start all 0, kv_total = kv_len, slots -1, nothing
+ * taken.  A row whose page number is outside [0, n_pages) gets slot -1 and
+ * sets the bounds bit.  Outputs may not overlap kv_len, new_len or n_free. */
+ARCLLM_CUDA_API int arcllm_cuda_paged_plan(const int32_t *kv_len, const int32_t *new_len, uint32_t n_requests,
+                                           uint32_t page_size, uint32_t n_pages, const int32_t *free_pages,
+                                           const int32_t *n_free, int32_t *block_table, uint32_t table_stride,
+                                           uint32_t max_rows, int32_t *row_start, int32_t *kv_total,
+                                           int32_t *positions, int32_t *slots, int32_t *n_free_out, void *stream);
+
+/* Rotary frequencies (angle per position of pair i, i < rot_dim / 2) in 64
+ * bits into freqs_host, and the factor on cos and sin into *attn_scale_host.
+ * Host-only arithmetic; the caller uploads freqs once.
+ *   NONE    theta^(-2i/rot_dim)
+ *   LINEAR  the same / factor
+ *   NTK     with theta * factor^(rot_dim / (rot_dim - 2)) in place of theta
+ *   YARN    pairs that turn more than 32 times over trained_ctx keep their
+ *           frequency, pairs that turn less than once get it / factor, a linear
+ *           ramp between; attn_scale = 0.1 ln(factor) + 1 (else 1). */
+enum arcllm_rope_scaling { ARC_ROPE_NONE = 0, ARC_ROPE_LINEAR = 1, ARC_ROPE_NTK = 2, ARC_ROPE_YARN = 3 };
+ARCLLM_CUDA_API int arcllm_cuda_rope_freqs(int scaling, uint32_t rot_dim, double theta, double factor,
+                                           double trained_ctx, double *freqs_host, float *attn_scale_host);
+
+/* For each row with slots[row] >= 0: adds the biases (fp32, each nullable) to
+ * q [q_heads*head_dim], k and v [kv_heads*head_dim], rotates the first rot_dim
+ * dims of every q and k head by positions[row] * freqs, and writes q to q_out
+ * and k, v to their slot of the cache, all rounded to the cache's type.  Rows
+ * with slot -1 are skipped (q_out is left as it was); a slot past the cache or
+ * a negative position is skipped too and sets the bounds bit.
+ *   act_type   of q, k, v: ARC_GGML_F32, F16 or BF16; row strides in elements
+ *              (a fused projection's output can be used in place);
+ *   layout     pairs (2i, 2i+1) as arcllm_cuda_rope_kv_rows, or (i, i + rot_dim/2);
+ *   freqs      rot_dim/2 doubles (device).
+ * Angles are formed in 64 bits, so positions are not limited by a table.
+ * q_out may be q itself (same type, same stride).  Slots must differ from one
+ * another.  16-byte aligned rows and rot_dim, head_dim % 16 == 0 take the
+ * vector form. */
+enum arcllm_rope_layout { ARC_ROPE_INTERLEAVED = 0, ARC_ROPE_HALVES = 1 };
+ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint64_t q_stride, const void *k,
+                                              uint64_t k_stride, const void *v, uint64_t v_stride, const float *bq,
+                                              const float *bk, const float *bv, const double *freqs, uint32_t rot_dim,
+                                              int layout, float attn_scale, const int32_t *positions,
+                                              const int32_t *slots, uint32_t rows, uint32_t q_heads,
+                                              const arcllm_cuda_paged_kv *kv, void *q_out, uint64_t q_out_stride,
+                                              void *stream);
+
+/* Causal attention of every request's new rows over its pages, those of the
+ * new rows among them (arcllm_cuda_attention_decode and
+ * arcllm_cuda_attention_prefill over pages, for any mixture of single tokens
+ * and chunks).  Row row_start[r] + i of request r stands at position
+ * p = kv_total[r] - n + i, n its number of rows, and sees positions j <= p;
+ * with window > 0 only those with j > p - window or j < sinks.
+ *   q, out       [max_rows][q_heads*head_dim] of the cache's type, row strides
+ *                in elements; rows of no request are left as they were;
+ *   block_table  as arcllm_cuda_paged_plan leaves it; entries of pages that no
+ *                row sees (before the window) are not read as pages' numbers;
+ *   max_new      at least the largest number of rows of one request;
+ *   scale        on q.k, > 0 (1/sqrt(head_dim) unless the model says otherwise);
+ *   workspace    arcllm_cuda_attention_paged_workspace bytes, any content;
+ *                calls that may overlap in time need one each.
+ * head_dim 64 or 128, q_heads/kv_heads 1..16, page_size a multiple of 16,
+ * n_requests <= 4096; pointers 16-byte aligned, strides multiples of 8.
+ * A request whose lengths do not fit (kv_total < n, n > max_new, a table row
+ * too short, rows past max_rows) is skipped and sets the bounds bit; a page
+ * number outside [0, n_pages) sets it too and reads as zeros. */
+ARCLLM_CUDA_API int arcllm_cuda_attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                                          uint64_t *out);
+ARCLLM_CUDA_API int arcllm_cuda_attention_paged(const void *q, uint64_t q_stride, const arcllm_cuda_paged_kv *kv,
+                                                const int32_t *block_table, uint32_t table_stride,
+                                                const int32_t *row_start, const int32_t *kv_total,
+                                                uint32_t n_requests, uint32_t max_rows, uint32_t max_new,
+                                                uint32_t q_heads, float scale, uint32_t window, uint32_t sinks,
+                                                void *out, uint64_t out_stride, void *workspace,
+                                                uint64_t workspace_bytes, void *stream);
+
+/* Sampling constraints on n_rows rows of logits [vocab] and the greedy choice
+ * (arcllm_cuda_argmax for a batch, on the device).  In this order, each step
+ * rounded to fp32 by itself:
+ *   token in the row's history:    l = l > 0 ? l / repetition : l * repetition;
+ *   generated count times:         l -= frequency * count;
+ *   generated at least once:       l -= presence;
+ *   an entry in the row's biases:  l += value (of several for one token the
+ *                                  last one counts);
+ *   mask bit 0:                    l = -inf.
+ *   history      [n_rows][history_stride] tokens; [0, prompt_len) is the prompt
+ *                (prompt_len null: none), [prompt_len, total_len) generated;
+ *                values outside the vocabulary are passed over;
+ *   repetition, frequency, presence  [n_rows], each nullable;
+ *   bias_start   [n_rows + 1] into bias_ids and bias_values; null: none;
+ *   mask         [n_rows][mask_stride] words, bit t % 32 of word t / 32 set:
+ *                token t is allowed; null: all are;
+ *   out          of the logits' type (F32, F16 or BF16), rounded to it; may be
+ *                logits itself with the same stride;
+ *   best         [n_rows] lowest index of the largest finite value of out, -1
+ *                when there is none; null: not wanted. */
+ARCLLM_CUDA_API int arcllm_cuda_logits_process(int type, const void *logits, uint64_t stride, uint32_t n_rows,
+                                               uint32_t vocab, const int32_t *history, uint32_t history_stride,
+                                               const int32_t *prompt_len, const int32_t *total_len,
+                                               const float *repetition, const float *frequency,
+                                               const float *presence, const int32_t *bias_start,
+                                               const int32_t *bias_ids, const float *bias_values,
+                                               const uint32_t *mask, uint32_t mask_stride, void *out,
+                                               uint64_t out_stride, int32_t *best, void *stream);
 
 /* ---- device memory and streams (for hosts that do not link the CUDA runtime) --- */
 /* Launch overlap for the calling thread (programmatic dependent launch, as the
