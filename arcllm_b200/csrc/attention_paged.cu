@@ -21,10 +21,10 @@ namespace {
 using namespace paged;
 
 // ---- few rows: one warp per stretch ------------------------------------------
-constexpr uint32_t kRowWarps = 8, kRowTile = 16, kRowMax = 16;  // packed rows of an item
+constexpr uint32_t kRowWarps = 8, kRowTile = 16;
 
 struct Segment {  // an unfinished item of a warp
-    uint32_t valid, u0, u1, r, kvh, mt;
+    uint32_t valid, u0, u1, r, kvh;
 };
 
 template <bool BF16>
@@ -53,44 +53,25 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                  : "memory");
 }
 
-// Query rows of an item: as many as fit kRowMax packed rows.
-__host__ __device__ __forceinline__ uint32_t rows_per_item(uint32_t gq) { return kRowMax / gq; }
-
-// Position in the line of units: request, KV head, row group, tile.
+// Position in the line of units: request, KV head, tile.
 struct Cursor {
-    uint32_t r, kvh, mt, i, mts, nt;
+    uint32_t r, kvh, i;
     Req q;
     Span s;
     __device__ __forceinline__ void enter(const Args& a) {  // request r's sizes
         bool bad = false;
         load_req(a, r, q, bad);
-        const uint32_t rpi = rows_per_item(a.gq);
-        mts = (q.n + rpi - 1u) / rpi;
         s = span_of<kRowTile>(a, q.p0, q.p0 + q.n - 1u);
-        nt = s.n;
     }
     __device__ __forceinline__ void seek(const Args& a, const uint32_t* off, uint32_t u) {
-        uint32_t lo = 0, hi = a.n_requests;
-        while (hi - lo > 1u) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (off[mid] <= u)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        r = lo;
+        r = request_of(off, a.n_requests, u);
         enter(a);
-        uint32_t rem = u - off[r];
-        i = rem % nt;
-        rem /= nt;
-        mt = rem % mts;
-        kvh = rem / mts;
+        kvh = (u - off[r]) / s.n;
+        i = u - off[r] - kvh * s.n;
     }
     __device__ __forceinline__ void next(const Args& a, const uint32_t* off) {
-        if (++i < nt) return;
+        if (++i < s.n) return;
         i = 0;
-        if (++mt < mts) return;
-        mt = 0;
         if (++kvh < a.kv_heads) return;
         kvh = 0;
         const uint32_t end = off[r + 1];
@@ -99,43 +80,6 @@ struct Cursor {
         if (r < a.n_requests) enter(a);
     }
 };
-
-// Units of every request before request r, in off[0 .. n]; all threads of the
-// CTA.  Returns the total, or 0 where it does not fit 31 bits.
-template <typename Units>
-__device__ __forceinline__ uint32_t scan_units(const Args& a, uint32_t* off, unsigned int* err, Units units) {
-    __shared__ unsigned long long s_warp[32];
-    __shared__ int s_bad;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if (threadIdx.x == 0) s_bad = 0, off[0] = 0;
-    unsigned long long base = 0;
-    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += blockDim.x) {
-        const uint32_t r = r0 + threadIdx.x;
-        bool bad = false;
-        unsigned long long v = 0;
-        if (r < a.n_requests) v = units(r, bad);
-        __syncthreads();
-        if (bad) s_bad = 1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= (uint32_t)o) v += x;
-        }
-        if (lane == 31u) s_warp[warp] = v;
-        __syncthreads();
-        unsigned long long all = 0;
-        for (uint32_t w = 0; w < warps; ++w) {
-            if (w < warp) v += s_warp[w];
-            all += s_warp[w];
-        }
-        if (r < a.n_requests) off[r + 1] = (uint32_t)(base + v);
-        base += all;
-    }
-    __syncthreads();
-    const bool too_many = base > 0x7fffffffull;
-    if (threadIdx.x == 0 && blockIdx.x == 0 && (s_bad || too_many)) raise_error(err, ARC_DEV_ERR_BOUNDS);
-    return too_many ? 0u : (uint32_t)base;
-}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowWarps * 32, 1)
@@ -159,12 +103,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
     fence_mbar_init();
     pdl_trigger();
     pdl_wait();  // lengths, queries and pages come from the preceding kernels
-    const uint32_t rpi = rows_per_item(a.gq);
     const uint32_t total = scan_units(a, off, err, [&](uint32_t r, bool& bad) -> unsigned long long {
         Req q;
-        if (!load_req(a, r, q, bad)) return 0;
-        return (unsigned long long)a.kv_heads * ((q.n + rpi - 1u) / rpi) *
-               span_of<kRowTile>(a, q.p0, q.p0 + q.n - 1u).n;
+        if (!load_req(a, r, q, bad) || q.n * a.gq > kRowMax) return 0;
+        return (unsigned long long)a.kv_heads * span_of<kRowTile>(a, q.p0, q.p0 + q.n - 1u).n;
     });
     // equal shares of whole rounds of the CTA's warps
     const uint32_t per = max(((total + gridDim.x - 1u) / gridDim.x + kRowWarps - 1u) / kRowWarps, 1u) * kRowWarps;
@@ -223,13 +165,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             if (it == 0 || cc.i == 0) {  // a new item: its queries into A fragments
                 seg_u0 = u0 + it;
                 first_seg = it == 0;
-                const uint32_t q0 = cc.mt * rpi;
-                item_rows = min(rpi, cc.q.n - q0) * a.gq;
-                item_row0 = cc.q.row0 + q0;
+                item_rows = cc.q.n * a.gq;
+                item_row0 = cc.q.row0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t ri = min(g + 8u * h, item_rows - 1u), qr = ri / a.gq;
-                    pos_of[h] = cc.q.p0 + q0 + qr;
+                    pos_of[h] = cc.q.p0 + qr;
                     const uint16_t* src = a.q + (uint64_t)(item_row0 + qr) * a.q_stride +
                                           (cc.kvh * a.gq + ri - qr * a.gq) * D + 2u * t;
 #pragma unroll
@@ -320,7 +261,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             __syncwarp();
             s_cons = s_cons + 1u == stages ? 0u : s_cons + 1u;
             if (s_cons == 0) parity ^= 1u;
-            const bool ends = cc.i + 1u == cc.nt;
+            const bool ends = cc.i + 1u == cc.s.n;
             if (issued < n_units) issue();
             if (ends || it + 1u == n_units) {
 #pragma unroll
@@ -355,7 +296,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
                         if (t == 0)
                             *reinterpret_cast<float2*>(slot + slot_rows * D + 2u * ri) = make_float2(m[h], l[h]);
                     }
-                    if (lane == 0) segs[warp][first_seg ? 0 : 1] = {1u, item_u0, item_u0 + cc.nt, cc.r, cc.kvh, cc.mt};
+                    if (lane == 0) segs[warp][first_seg ? 0 : 1] = {1u, item_u0, item_u0 + cc.s.n, cc.r, cc.kvh};
                 }
             }
             if (it + 1u < n_units) cc.next(a, off);
@@ -382,12 +323,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
         Req q;
         bool bad = false;
         load_req(a, sg.r, q, bad);
-        const uint32_t q0 = sg.mt * rpi, rows = min(rpi, q.n - q0) * a.gq;
+        const uint32_t rows = q.n * a.gq;
         const bool whole = sg.u0 >= U0 && sg.u1 <= U1;
         const uint32_t slot_no = sg.u0 < U0 ? 0u : 1u;
         float* part = parts + (uint64_t)(blockIdx.x * 2u + slot_no) * (kRowMax * (D + 2u));
         if (!whole && slot_no == 1u && tid == 0)
-            recs[blockIdx.x] = {1u, (sg.u1 - 1u) / per, q.row0 + q0, rows, sg.kvh, {0, 0, 0}};
+            recs[blockIdx.x] = {1u, (sg.u1 - 1u) / per, q.row0, rows, sg.kvh, {0, 0, 0}};
         for (uint32_t x = tid; x < rows * (D / 4u); x += kRowWarps * 32u) {
             const uint32_t ri = x / (D / 4u), c = (x - ri * (D / 4u)) * 4u;
             float M = -INFINITY;
@@ -414,7 +355,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             if (whole) {
                 const uint32_t qr = ri / a.gq;
                 const float inv = 1.f / L;
-                *reinterpret_cast<uint2*>(a.out + (uint64_t)(q.row0 + q0 + qr) * a.out_stride +
+                *reinterpret_cast<uint2*>(a.out + (uint64_t)(q.row0 + qr) * a.out_stride +
                                           (sg.kvh * a.gq + ri - qr * a.gq) * D + c) =
                     make_uint2(pack16<BF16>(A.x * inv, A.y * inv), pack16<BF16>(A.z * inv, A.w * inv));
             } else {
@@ -427,21 +368,26 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 }
 
 // ---- join ---------------------------------------------------------------------
-// Block (c, part): the item that CTA c began and later CTAs went on with.
+// Block (c, part): the item that CTA c began and later CTAs went on with.  The
+// first kSms records are the rows kernel's, the others the tile kernel's.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Record* __restrict__ recs,
-                                                              const float* __restrict__ parts, uint32_t max_rows) {
+                                                              const float* __restrict__ row_parts,
+                                                              const float* __restrict__ tile_parts, uint32_t rec0) {
     pdl_trigger();
     pdl_wait();
-    const Record rc = recs[blockIdx.x];
+    const Record rc = recs[rec0 + blockIdx.x];
     if (!rc.valid) return;
-    const uint32_t stride = max_rows * (D + 2u);
+    const bool tiles = rec0 + blockIdx.x >= kSms;
+    const uint32_t cta = rec0 + blockIdx.x - (tiles ? kSms : 0u);
+    const uint32_t max_rows = tiles ? kTileRows : kRowMax, stride = max_rows * (D + 2u);
+    const float* parts = tiles ? tile_parts : row_parts;
     for (uint32_t x = blockIdx.y * blockDim.x + threadIdx.x; x < rc.rows * (D / 4u); x += gridDim.y * blockDim.x) {
         const uint32_t ri = x / (D / 4u), c = (x - ri * (D / 4u)) * 4u;
         constexpr uint32_t CH = 8;  // parts whose loads are in flight together
         float M = -INFINITY, L = 0.f;
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t j0 = blockIdx.x; j0 <= rc.last_cta; j0 += CH) {
+        for (uint32_t j0 = cta; j0 <= rc.last_cta; j0 += CH) {
             float2 ml[CH];
             float4 v[CH];
 #pragma unroll
@@ -449,7 +395,7 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Reco
                 ml[j] = make_float2(-INFINITY, 0.f);
                 v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (j0 + j <= rc.last_cta) {
-                    const float* p = parts + (uint64_t)((j0 + j) * 2u + (j0 + j == blockIdx.x ? 1u : 0u)) * stride;
+                    const float* p = parts + (uint64_t)((j0 + j) * 2u + (j0 + j == cta ? 1u : 0u)) * stride;
                     ml[j] = *reinterpret_cast<const float2*>(p + max_rows * D + 2u * ri);
                     v[j] = *reinterpret_cast<const float4*>(p + ri * D + c);
                 }
@@ -478,15 +424,49 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Reco
 }
 
 // ---- host ---------------------------------------------------------------------
-struct Workspace {
-    Record* recs;
-    float* parts;
-};
-constexpr uint64_t kRecBytes = (sizeof(Record) * kSms + 255u) / 256u * 256u;
-uint64_t rows_part_bytes(uint32_t d) { return 4ull * kSms * 2u * kRowMax * (d + 2u); }
+// Workspace: the records of both kernels, then their parts.
+constexpr uint64_t kRecBytes = (sizeof(Record) * 2u * kSms + 255u) / 256u * 256u;
+constexpr uint64_t rows_part_bytes(uint32_t d) { return 4ull * kSms * 2u * kRowMax * (d + 2u); }
 
-// Tensor map of K or V: boxes of `tokens` positions x 64 dims of one head of one page, 128-byte swizzle.
-int encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens) {
+template <int D, bool BF16>
+int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args& a, cudaStream_t stream) {
+    constexpr uint32_t kStage = 4u * kRowTile * D, kMost = 232448u - 2048u;  // 227 KB less the static arrays
+    uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+    Record* recs = reinterpret_cast<Record*>(ws);
+    float* parts = reinterpret_cast<float*>(ws + kRecBytes);
+    float* tile_parts = reinterpret_cast<float*>(ws + kRecBytes + rows_part_bytes(D));
+    // the requests with few rows, if any can have; then those with many
+    const bool few = a.gq <= kRowMax, many = (uint64_t)a.max_new * a.gq > kRowMax;
+    cudaError_t e = cudaSuccess;
+    if (few) {
+        CUtensorMap kmap, vmap;
+        int st = encode_pages(&kmap, kv, kv.k_pages, kRowTile);
+        if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, kRowTile);
+        if (st != ARC_OK) return st;
+        const uint32_t slot_rows = !many && a.max_new * a.gq <= 8u ? 8u : 16u;
+        const uint32_t fixed = 1024u + kRowWarps * slot_rows * (D + 2u) * 4u + 4u * (a.n_requests + 1u);
+        const uint32_t stages = std::min(4u, (kMost - fixed) / (kRowWarps * kStage));
+        e = cudaFuncSetAttribute(attn_paged_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kMost);
+        if (e == cudaSuccess)
+            e = launch_kernel(attn_paged_rows_kernel<D, BF16>, dim3(kSms), dim3(kRowWarps * 32u),
+                              fixed + kRowWarps * stages * kStage, stream, kmap, vmap, a, slot_rows, stages, recs,
+                              parts, dev_error_word());
+    }
+    if (e == cudaSuccess && many) {
+        const int st = launch_tiles<D, BF16>(kv, a, recs + kSms, tile_parts, stream);
+        if (st != ARC_OK) return st;
+    }
+    // blocks of the records that were written
+    if (e == cudaSuccess)
+        e = launch_kernel(attn_paged_join_kernel<D, BF16>, dim3((few ? kSms : 0u) + (many ? kSms : 0u), many ? 16 : 2),
+                          dim3(256), 0, stream, a, recs, parts, tile_parts, few ? 0u : kSms);
+    return launch_checked(e, "attention paged launch");
+}
+
+}  // namespace
+
+int paged::encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens) {
     const EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return set_error(ARC_E_CUDA, "attention paged: cuTensorMapEncodeTiled is not available");
     const cuuint64_t dims[4] = {kv.head_dim, kv.page_size, kv.kv_heads, kv.n_pages};
@@ -499,41 +479,13 @@ int encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* b
     return rc == CUDA_SUCCESS ? ARC_OK : set_error(ARC_E_CUDA, "attention paged: tensor map of the pages");
 }
 
-template <int D, bool BF16>
-int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args& a, cudaStream_t stream) {
-    constexpr uint32_t kStage = 4u * kRowTile * D, kMost = 232448u - 2048u;  // 227 KB less the static arrays
-    CUtensorMap kmap, vmap;
-    int st = encode_pages(&kmap, kv, kv.k_pages, kRowTile);
-    if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, kRowTile);
-    if (st != ARC_OK) return st;
-    uint8_t* ws = static_cast<uint8_t*>(p.workspace);
-    Record* recs = reinterpret_cast<Record*>(ws);
-    float* parts = reinterpret_cast<float*>(ws + kRecBytes);
-    const uint32_t rpi = rows_per_item(a.gq);
-    const uint32_t slot_rows = std::min(rpi, a.max_new) * a.gq <= 8u ? 8u : 16u;
-    const uint32_t fixed = 1024u + kRowWarps * slot_rows * (D + 2u) * 4u + 4u * (a.n_requests + 1u);
-    const uint32_t stages = std::min(4u, (kMost - fixed) / (kRowWarps * kStage));
-    const uint32_t smem = fixed + kRowWarps * stages * kStage;
-    cudaError_t e = cudaFuncSetAttribute(attn_paged_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)kMost);
-    if (e == cudaSuccess)
-        e = launch_kernel(attn_paged_rows_kernel<D, BF16>, dim3(kSms), dim3(kRowWarps * 32u), smem, stream, kmap, vmap,
-                          a, slot_rows, stages, recs, parts, dev_error_word());
-    if (e == cudaSuccess)
-        e = launch_kernel(attn_paged_join_kernel<D, BF16>, dim3(kSms, 2), dim3(256), 0, stream, a, recs, parts,
-                          kRowMax);
-    return launch_checked(e, "attention paged launch");
-}
-
-}  // namespace
-
 int attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint64_t* out) {
     if (!out) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged workspace: null out");
     if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged workspace: q_heads % kv_heads");
     if (head_dim != 64u && head_dim != 128u)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged workspace: head_dim must be 64 or 128");
-    *out = kRecBytes + rows_part_bytes(head_dim);
+    *out = kRecBytes + rows_part_bytes(head_dim) + 4ull * kSms * 2u * kTileRows * (head_dim + 2u);
     return ARC_OK;
 }
 
@@ -545,7 +497,7 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
     const int st = attention_paged_workspace(p.q_heads, kv.kv_heads, kv.head_dim, &need);
     if (st != ARC_OK) return st;
     const uint32_t gq = p.q_heads / kv.kv_heads;
-    if (gq > 16u) return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 16 query heads per KV head");
+    if (gq > 128u) return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 128 query heads per KV head");
     if (kv.page_size % 16u) return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: page_size must be a multiple of 16");
     if (p.n_requests > kMaxRequests)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 4096 requests");

@@ -14,6 +14,8 @@ namespace arc {
 namespace paged {
 
 constexpr uint32_t kSms = 148;          // one CTA per SM in both attention kernels
+constexpr uint32_t kTileRows = 256;     // packed rows of an item of the tile kernel
+constexpr uint32_t kRowMax = 16;        // requests with at most so many packed rows go to the rows kernel
 constexpr uint32_t kMaxRequests = 4096; // unit offsets of the requests in shared memory
 
 struct Args {
@@ -92,6 +94,56 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return r;
 }
 
+// The request that unit u of the line belongs to.
+__device__ __forceinline__ uint32_t request_of(const uint32_t* off, uint32_t n, uint32_t u) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (off[mid] <= u)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// Units of every request before request r, in off[0 .. n]; all threads of the
+// CTA.  Returns the total, or 0 where it does not fit 31 bits.
+template <typename Units>
+__device__ __forceinline__ uint32_t scan_units(const Args& a, uint32_t* off, unsigned int* err, Units units) {
+    __shared__ unsigned long long s_warp[32];
+    __shared__ int s_bad;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (threadIdx.x == 0) s_bad = 0, off[0] = 0;
+    unsigned long long base = 0;
+    for (uint32_t r0 = 0; r0 < a.n_requests; r0 += blockDim.x) {
+        const uint32_t r = r0 + threadIdx.x;
+        bool bad = false;
+        unsigned long long v = 0;
+        if (r < a.n_requests) v = units(r, bad);
+        __syncthreads();
+        if (bad) s_bad = 1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long x = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= (uint32_t)o) v += x;
+        }
+        if (lane == 31u) s_warp[warp] = v;
+        __syncthreads();
+        unsigned long long all = 0;
+        for (uint32_t w = 0; w < warps; ++w) {
+            if (w < warp) v += s_warp[w];
+            all += s_warp[w];
+        }
+        if (r < a.n_requests) off[r + 1] = (uint32_t)(base + v);
+        base += all;
+    }
+    __syncthreads();
+    const bool too_many = base > 0x7fffffffull;
+    if (threadIdx.x == 0 && blockIdx.x == 0 && (s_bad || too_many)) raise_error(err, ARC_DEV_ERR_BOUNDS);
+    return too_many ? 0u : (uint32_t)base;
+}
+
 // Box of the pages' tensor (dim, token, KV head, page) into shared memory; out of range reads zero.
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int dim, int token, int head, int page,
                                          uint64_t* bar) {
@@ -101,6 +153,14 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(token), "r"(head), "r"(page), "r"(smem_addr(bar))
         : "memory");
 }
+
+// Tensor map of K or V: boxes of `tokens` positions x 64 dims of one head of one page, 128-byte swizzle.
+int encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens);
+
+// The requests with more than kRowMax packed rows (attention_paged_tiles.cu).
+template <int D, bool BF16>
+int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, float* parts,
+                 cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace arc

@@ -1,0 +1,509 @@
+// Paged attention of requests with many new rows on the 5th-generation tensor
+// cores (B200, sm_100a).
+//
+// An item is one KV head and up to 2 x 128 packed rows ((row, head of the
+// group) pairs, whole rows); a unit is a tile of 128 positions.  Per item and
+// tile, for each half s of the rows:
+//   S_s = Q_s K^T        tcgen05.mma, both operands in shared memory
+//   P_s = exp2(S_s - m)  one thread per row: S out of tensor memory, the row's
+//                        maximum and sum in registers, P back over S in 16 bits
+//   O_s += P_s V         tcgen05.mma, P in tensor memory, V in shared memory
+// The halves alternate: while one half's softmax runs, the tensor core works
+// on the other's products.
+//   warps 0..3, 4..7  softmax of half 0, 1: also load Q, write the output
+//   warp 8            TMA: pages' K and V rows into a ring of tiles
+//   warp 9            issues the MMAs (10 and 11 only complete the warpgroup)
+// O is scaled only when a row's maximum has grown by more than 2^8 since the
+// last time (the sums carry the same factor, so the result is the same); MMAs
+// of one thread run in order, so when S of a tile is there, all products
+// before it are done and O may be touched, and P may lie over S.
+// K and V tiles are built from boxes of a power of two of positions that
+// divides the page, so tiles and pages need not match.
+// All waits are bounded: on a timeout the roles leave their loops, drain what
+// they started and the error word is set.
+#include <algorithm>
+
+#include "arcllm_cuda_internal.h"
+#include "attention_paged.cuh"
+#include "tmem.cuh"
+
+namespace arc {
+namespace paged {
+namespace {
+
+constexpr uint32_t kTile = 128;  // positions
+constexpr uint32_t kThreads = 384;
+// Registers: the softmax threads hold a row of S.  (8 x 208 + 4 x 80) x 32 <= 384 x 168, what the block starts with.
+constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that is let pass
+
+template <int D>
+struct Layout {
+    static constexpr uint32_t kHalves = D / 64;               // 64-dim columns of 128 rows x 128 bytes
+    static constexpr uint32_t kBytes = kHalves * 16384u;      // a Q half, a K tile or a V tile
+    static constexpr uint32_t kStages = 4u * 128u / D;        // K and V tiles in the ring: 128 KB
+    static constexpr uint32_t kRing = 2u * kBytes;            // after the two Q halves
+    static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
+};
+
+// The item that a role is at, and the part of its tiles that this CTA does.
+struct Walk {
+    uint32_t r, kvh, mt, i, left;  // left: units of the CTA's stretch from here on
+    uint32_t n_items;              // of the request
+    Req q;
+    uint32_t first, rows;  // query rows [first, first + rows) of the request
+    uint32_t lo, hi;       // their positions
+    Span s;
+    __device__ __forceinline__ void enter(const Args& a, uint32_t per_item) {
+        bool bad = false;
+        load_req(a, r, q, bad);
+        n_items = (q.n + per_item - 1u) / per_item;
+    }
+    __device__ __forceinline__ void item(const Args& a, uint32_t per_item) {
+        first = mt * per_item;
+        rows = min(per_item, q.n - first);
+        lo = q.p0 + first;
+        hi = lo + rows - 1u;
+        s = span_of<kTile>(a, lo, hi);
+    }
+    __device__ __forceinline__ uint32_t end() const { return min(s.n, i + left); }
+    __device__ __forceinline__ bool next(const Args& a, const uint32_t* off, uint32_t per_item) {
+        left -= end() - i;
+        if (left == 0) return false;
+        i = 0;
+        if (++mt == n_items) {
+            mt = 0;
+            if (++kvh == a.kv_heads) {
+                kvh = 0;
+                const uint32_t e = off[r + 1];
+                do ++r;
+                while (off[r + 1] == e);  // units are left, so a request with units follows
+                enter(a, per_item);
+            }
+        }
+        item(a, per_item);
+        return true;
+    }
+};
+
+__device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint32_t mt, uint32_t per_item) {
+    const uint32_t first = mt * per_item, rows = min(per_item, q.n - first);
+    return span_of<kTile>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
+}
+
+// A role's wait: false once any role has given up.  The same for all lanes.
+__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
+    const bool here = mbar_wait(bar, parity, err) && !*abort_flag;
+    return __all_sync(0xffffffffu, here);
+}
+
+// Positions at, of a tile, that some row of the item sees (lo, hi its positions).
+__device__ __forceinline__ bool any_sees(const Args& a, uint32_t lo, uint32_t hi, uint32_t at) {
+    return at <= hi && (a.window == 0u || at + a.window > lo || at < a.sinks);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a,
+                            uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
+                            unsigned int* err) {
+    using L = Layout<D>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
+    uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
+    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], s_full[2], p_full[2], o_full[2], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int abort_flag;
+    __shared__ uint32_t start[4];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    if (tid == 0) {
+        for (uint32_t s = 0; s < L::kStages; ++s) mbar_init(&kv_full[s], 1), mbar_init(&kv_empty[s], 1);
+        for (uint32_t s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], 4);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 4);
+            mbar_init(&o_full[s], 1);
+        }
+        mbar_init(&done, 1);
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_base)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_trigger();
+    pdl_wait();  // lengths, queries and pages come from the preceding kernels
+
+    // The CTA's stretch.  Units of every request: by its thread where it has few items, by a warp otherwise.
+    const uint32_t half_rows = 128u / a.gq, per_item = 2u * half_rows;
+    constexpr uint32_t kAlone = 8, kMany = 0xffffffffu;
+    bool any_bad = false;
+    for (uint32_t r = tid; r < a.n_requests; r += kThreads) {
+        Req q;
+        unsigned long long u = 0;
+        if (load_req(a, r, q, any_bad) && q.n * a.gq > kRowMax) {
+            const uint32_t items = (q.n + per_item - 1u) / per_item;
+            if (items <= kAlone) {
+                for (uint32_t mt = 0; mt < items; ++mt) u += item_units(a, q, mt, per_item);
+                u = min(u * a.kv_heads, 0xfffffffeull);
+            } else {
+                u = kMany;
+            }
+        }
+        off[r + 1] = (uint32_t)u;
+    }
+    __syncthreads();
+    for (uint32_t r = warp; r < a.n_requests; r += kThreads / 32u) {
+        if (off[r + 1] != kMany) continue;
+        Req q;
+        bool bad = false;
+        load_req(a, r, q, bad);
+        const uint32_t items = (q.n + per_item - 1u) / per_item;
+        unsigned long long u = 0;
+        for (uint32_t mt = lane; mt < items; mt += 32u) u += item_units(a, q, mt, per_item);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        if (lane == 0) off[r + 1] = (uint32_t)min(u * a.kv_heads, 0xfffffffeull);
+    }
+    __syncthreads();
+    const uint32_t total = scan_units(a, off, err, [&](uint32_t r, bool& bad) -> unsigned long long {
+        bad = any_bad;
+        return off[r + 1];
+    });
+    const uint32_t per = max((total + gridDim.x - 1u) / gridDim.x, least);
+    const uint32_t U0 = (uint32_t)min((unsigned long long)blockIdx.x * per, (unsigned long long)total);
+    const uint32_t n_units = min(per, total - U0);
+    if (tid == 0) recs[blockIdx.x].valid = 0;
+    if (n_units != 0 && warp == 10) {
+        const uint32_t r = request_of(off, a.n_requests, U0);
+        Req q;
+        bool bad = false;
+        load_req(a, r, q, bad);
+        const uint32_t head = (off[r + 1] - off[r]) / a.kv_heads, kvh = (U0 - off[r]) / head;
+        uint32_t rem = U0 - off[r] - kvh * head, mt = 0;
+        const uint32_t items = (q.n + per_item - 1u) / per_item;
+        for (uint32_t m0 = 0; m0 < items; m0 += 32u) {  // the item that unit rem of the head lies in
+            uint32_t v = m0 + lane < items ? item_units(a, q, m0 + lane, per_item) : 0u;
+            const uint32_t mine = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= (uint32_t)o) v += x;
+            }
+            const uint32_t over = __ballot_sync(0xffffffffu, v > rem);
+            if (over) {
+                const int at = __ffs(over) - 1;
+                mt = m0 + (uint32_t)at;
+                rem -= __shfl_sync(0xffffffffu, v - mine, at);
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) start[0] = r, start[1] = kvh, start[2] = mt, start[3] = rem;
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    Walk w;
+    if (n_units != 0) {
+        w.r = start[0], w.kvh = start[1], w.mt = start[2], w.i = start[3], w.left = n_units;
+        w.enter(a, per_item);
+        w.item(a, per_item);
+    }
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      if (n_units == 0) {
+        // nothing to do; the tensor memory is given back below
+      } else if (warp == 8) {
+        // ---------------- TMA: K, V, K, V ... tile by tile ----------------
+        const uint32_t boxes = kTile / box;
+        uint32_t stage = 0, phase = 0, issued = 0;
+        bool bad_page = false, ok = true;
+        do {
+            for (uint32_t i = w.i; i < w.end() && ok; ++i) {
+                const uint32_t p = w.s.tile(i) * kTile + lane * box;  // lane b: box b of the tile
+                bool need = false;
+                int page = 0;
+                if (lane < boxes) {  // a box is loaded when it holds anything seen
+                    const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
+                    need = p <= w.hi && (p + box > from || p < a.sinks);
+                    if (need) page = a.table[(uint64_t)w.r * a.table_stride + p / a.page_size];
+                    if ((uint32_t)page >= a.n_pages) bad_page = true, page = (int)a.n_pages;  // reads zeros
+                }
+                const uint32_t n_need = __popc(__ballot_sync(0xffffffffu, need));
+#pragma unroll
+                for (uint32_t kv = 0; kv < 2; ++kv) {
+                    if (issued >= L::kStages) ok = role_wait(&kv_empty[stage], phase ^ 1u, &abort_flag, err);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], n_need * L::kHalves * box * 128u);
+                    __syncwarp();
+                    if (need) {
+                        uint8_t* dst = smem + L::kRing + stage * L::kBytes + lane * box * 128u;
+#pragma unroll
+                        for (uint32_t h = 0; h < L::kHalves; ++h)
+                            tma_page(dst + h * 16384u, kv ? &vmap : &kmap, (int)(64u * h), (int)(p % a.page_size),
+                                     (int)w.kvh, page, &kv_full[stage]);
+                    }
+                    ++issued;
+                    if (++stage == L::kStages) stage = 0, phase ^= 1u;
+                }
+            }
+        } while (ok && w.next(a, off, per_item));
+        if (!ok) {  // no copy may still be landing at the end
+            abort_flag = 1;
+            for (uint32_t k = issued > L::kStages ? issued - L::kStages : 0u; k < issued; ++k)
+                mbar_wait(&kv_full[k % L::kStages], (k / L::kStages) & 1u, err);
+        }
+        if (__any_sync(0xffffffffu, bad_page) && lane == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
+      } else if (warp == 9) {
+        // ---------------- MMA ----------------
+        constexpr uint32_t kQk = instr_desc<BF16>(128, false), kPv = instr_desc<BF16>(D, true);
+        const uint32_t ring = smem_addr(smem + L::kRing), qs = smem_addr(smem);
+        uint32_t stage = 0, phase = 0, n_item[2] = {0, 0}, n_s[2] = {0, 0};
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = role_wait(bar, parity, &abort_flag, err); };
+        auto qk = [&](uint32_t s, uint32_t k_stage) {
+            const uint64_t qa = operand_desc(qs + s * L::kBytes, 16u), kb = operand_desc(ring + k_stage * L::kBytes, 16u);
+#pragma unroll
+            for (uint32_t kk = 0; kk < D / 16u; ++kk) {
+                const uint32_t o = ((kk >> 2) * 16384u + (kk & 3u) * 32u) >> 4;  // addresses count 16 bytes
+                mma_smem(tmem + s * 128u, qa + o, kb + o, kQk, kk != 0u);
+            }
+            mma_commit(&s_full[s]);
+        };
+#pragma unroll 1
+        do {
+            const uint32_t i0 = w.i, i1 = w.end(), subs = w.rows > half_rows ? 2u : 1u;
+            // S of the first tile
+            if (!wait(&kv_full[stage], phase)) break;
+            
+#pragma unroll 1
+for (uint32_t s = 0; s < subs && ok; ++s) {
+                if (!wait(&q_full[s], n_item[s] & 1u)) break;
+                ++n_item[s];
+                tmem_fence_after();
+                if (lane == 0) qk(s, stage);
+            }
+            if (!ok) break;
+            if (lane == 0) mma_commit(&kv_empty[stage]);
+            if (++stage == L::kStages) stage = 0, phase ^= 1u;
+            for (uint32_t i = i0; i < i1 && ok; ++i) {
+                const uint32_t v_stage = stage;
+                const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 16384u);
+                if (!wait(&kv_full[v_stage], phase)) break;
+                if (++stage == L::kStages) stage = 0, phase ^= 1u;
+                // V rows of positions that no row of the item sees are zeroed: what lies there may be anything,
+                // and the weight 0 does not stop a NaN.
+                const uint32_t p0 = w.s.tile(i) * kTile;
+                const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
+                if (p0 + kTile - 1u > w.hi || (p0 < from && p0 + kTile > a.sinks)) {
+#pragma unroll 1
+                    for (uint32_t r = 0; r < kTile; r += 4u) {  // 8 lanes a row of 128 bytes
+                        const uint32_t row = r + (lane >> 3);
+                        if (!any_sees(a, w.lo, w.hi, p0 + row))
+#pragma unroll
+                            for (uint32_t h = 0; h < L::kHalves; ++h)
+                                *reinterpret_cast<uint4*>(smem + L::kRing + v_stage * L::kBytes + h * 16384u +
+                                                          row * 128u + (lane & 7u) * 16u) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                const bool more = i + 1u < i1;
+                
+#pragma unroll 1
+for (uint32_t s = 0; s < subs && ok; ++s) {
+                    if (!wait(&p_full[s], n_s[s] & 1u)) break;
+                    ++n_s[s];
+                    tmem_fence_after();
+                    if (lane == 0) {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
+                            mma_tmem(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u,
+                                     vb + kk * (2048u >> 4), kPv, i != i0 || kk != 0u);
+                        if (s + 1u == subs) mma_commit(&kv_empty[v_stage]);
+                    }
+                    if (more) {
+                        if (s == 0 && !wait(&kv_full[stage], phase)) break;
+                        if (lane == 0) {
+                            qk(s, stage);
+                            if (s + 1u == subs) mma_commit(&kv_empty[stage]);
+                        }
+                    } else if (lane == 0) {
+                        mma_commit(&o_full[s]);
+                    }
+                }
+                if (more && ok && ++stage == L::kStages) stage = 0, phase ^= 1u;
+            }
+        } while (ok && w.next(a, off, per_item));
+        if (!ok) abort_flag = 1;
+        if (lane == 0) mma_commit(&done);
+        __syncwarp();
+        mbar_wait(&done, 0, err);  // nothing of this CTA runs on the tensor core any more
+      }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+      if (n_units != 0) {
+        // ---------------- softmax of half s: thread t has packed row t ----------------
+        const uint32_t s = warp >> 2, t = tid & 127u;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+        const uint32_t ts = tmem + lanes + s * 128u, to = tmem + lanes + 256u + s * 128u;
+        uint8_t* qdst = smem + s * L::kBytes + (t >> 3) * 1024u + (t & 7u) * 128u;
+        uint32_t n_s = 0, n_o = 0, u = U0;
+        bool ok = true;
+        do {
+            const uint32_t i0 = w.i, i1 = w.end(), item_u0 = u - i0;
+            u += i1 - i0;
+            if (s * half_rows >= w.rows) continue;  // this half has no rows (uniform over its warps)
+            const uint32_t sub_rows = min(half_rows, w.rows - s * half_rows), packed = sub_rows * a.gq;
+            const uint32_t qr = min(t / a.gq, sub_rows - 1u);
+            const uint32_t pos = w.lo + s * half_rows + qr;
+            const uint64_t row = w.q.row0 + w.first + s * half_rows + qr;
+            const uint32_t col = (w.kvh * a.gq + t % a.gq) * D;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.q_stride + col);
+#pragma unroll
+                for (uint32_t c = 0; c < D / 8u; ++c) {
+                    const uint4 v = t < packed ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(qdst + (c >> 3) * 16384u + (((c & 7u) ^ (t & 7u)) << 4)) = v;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tmem_fence_before();  // the last item's O has been read
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[s]);
+            }
+            const uint32_t p_lo = w.lo + s * half_rows, p_hi = p_lo + sub_rows - 1u;
+            float m = -INFINITY, l = 0.f;
+            for (uint32_t i = i0; i < i1; ++i) {
+                ok = role_wait(&s_full[s], n_s & 1u, &abort_flag, err);
+                if (!ok) break;
+                ++n_s;
+                tmem_fence_after();
+                float x[4][32];
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) tmem_ld32(ts + 32u * k, x[k]);
+                const uint32_t p0 = w.s.tile(i) * kTile;
+                if (p0 + kTile - 1u > p_lo ||
+                    (a.window && p0 + a.window <= p_hi && p0 + kTile > a.sinks)) {  // not all rows see all of it
+#pragma unroll
+                    for (uint32_t c = 0; c < 128u; ++c)
+                        if (!visible(a, pos, p0 + c)) x[c / 32u][c % 32u] = -INFINITY;
+                }
+                float mx[4] = {x[0][0], x[1][0], x[2][0], x[3][0]};
+#pragma unroll
+                for (uint32_t c = 1; c < 32u; ++c)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) mx[k] = fmaxf(mx[k], x[k][c]);
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+                if (i == i0) {
+                    m = mn;  // O is written afresh
+                } else if (__any_sync(0xffffffffu, mn > m + kGrow)) {
+                    const float to_m = fmaxf(m, mn);
+                    const float f = ex2(m - (to_m == -INFINITY ? 0.f : to_m));
+                    l *= f;
+                    m = to_m;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                        float o[32];
+                        tmem_ld32(to + c, o);
+                        uint32_t ob[32];
+#pragma unroll
+                        for (uint32_t k = 0; k < 32u; ++k) ob[k] = __float_as_uint(o[k] * f);
+                        tmem_st32(to + c, ob);
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < 128u; c0 += 64u) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (uint32_t c = 0; c < 64u; c += 2u) {
+                        const float e0 = ex2(fmaf(x[(c0 + c) / 32u][c % 32u], a.scale_log2, -ref));
+                        const float e1 = ex2(fmaf(x[(c0 + c) / 32u][c % 32u + 1u], a.scale_log2, -ref));
+                        sum[c & 2u] += e0, sum[(c & 2u) + 1u] += e1;
+                        // the product takes weights of the cache's type: half a step of it each, as the output
+                        pk[c / 2u] = pack16<BF16>(e0, e1);
+                    }
+                    tmem_st32(ts + c0 / 2u, pk);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[s]);
+            }
+            if (ok) ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
+            if (!ok) break;
+            ++n_o;
+            tmem_fence_after();
+            const bool whole = i0 == 0 && i1 == w.s.n;
+            const uint32_t slot = i0 != 0 ? 0u : 1u;  // began before this stretch, or goes on after it
+            float* part = parts + (uint64_t)(blockIdx.x * 2u + slot) * (kTileRows * (D + 2u));
+            const uint32_t ri = s * half_rows * a.gq + t;
+            const float inv = 1.f / l;
+#pragma unroll 1
+            for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
+                float o[32];
+                tmem_ld32(to + c, o);
+                if (t < packed && whole) {
+                    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + col + c);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k)
+                        dst[k] = make_uint4(pack16<BF16>(o[8 * k] * inv, o[8 * k + 1] * inv),
+                                            pack16<BF16>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                            pack16<BF16>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
+                                            pack16<BF16>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                } else if (t < packed) {
+                    float4* dst = reinterpret_cast<float4*>(part + (uint64_t)ri * D + c);
+#pragma unroll
+                    for (uint32_t k = 0; k < 8u; ++k)
+                        dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                }
+                __syncwarp();
+            }
+            if (!whole) {
+                if (t < packed) *reinterpret_cast<float2*>(part + kTileRows * D + 2u * ri) = make_float2(m, l);
+                if (slot == 1u && tid == 0)
+                    recs[blockIdx.x] = {1u, (item_u0 + w.s.n - 1u) / per, w.q.row0 + w.first, w.rows * a.gq, w.kvh,
+                                        {0, 0, 0}};
+            }
+        } while (w.next(a, off, per_item));
+        if (!ok) abort_flag = 1;
+      }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+}  // namespace
+
+template <int D, bool BF16>
+int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, float* parts, cudaStream_t stream) {
+    using L = Layout<D>;
+    uint32_t box = 16;  // the largest power of two up to the tile that divides the page
+    while (box < kTile && kv.page_size % (2u * box) == 0u) box *= 2u;
+    CUtensorMap kmap, vmap;
+    int st = encode_pages(&kmap, kv, kv.k_pages, box);
+    if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, box);
+    if (st != ARC_OK) return st;
+    const uint32_t smem = 1024u + L::kOff + 4u * (a.n_requests + 1u);
+    cudaError_t e = cudaFuncSetAttribute(attn_paged_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
+    if (e == cudaSuccess)
+        e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap, a,
+                          box, 1u, recs, parts, dev_error_word());
+    return e == cudaSuccess ? ARC_OK : set_cuda_error(e, "attention paged tiles launch");
+}
+
+template int launch_tiles<64, false>(const arcllm_cuda_paged_kv&, const Args&, Record*, float*, cudaStream_t);
+template int launch_tiles<64, true>(const arcllm_cuda_paged_kv&, const Args&, Record*, float*, cudaStream_t);
+template int launch_tiles<128, false>(const arcllm_cuda_paged_kv&, const Args&, Record*, float*, cudaStream_t);
+template int launch_tiles<128, true>(const arcllm_cuda_paged_kv&, const Args&, Record*, float*, cudaStream_t);
+
+}  // namespace paged
+}  // namespace arc
