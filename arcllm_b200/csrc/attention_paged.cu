@@ -83,12 +83,11 @@ struct Cursor {
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowWarps * 32, 1)
-    attn_paged_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a,
-                           uint32_t slot_rows, uint32_t stages, Record* __restrict__ recs, float* __restrict__ parts,
+    attn_paged_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                           PageMap heads, Args a, uint32_t slot_rows, uint32_t stages, Record* __restrict__ recs, float* __restrict__ parts,
                            unsigned int* err) {
-    constexpr uint32_t HB = kRowTile * 128u;           // one box: 16 positions x 64 dims
-    constexpr uint32_t NH = D / 64;                    // boxes per K or V tile
-    constexpr uint32_t TILE = NH * HB, STAGE = 2u * TILE;
+    constexpr uint32_t GB = D / 64 * 1024u;  // 8 positions: [64-dim part][8][128 bytes]
+    constexpr uint32_t TILE = kRowTile / 8u * GB, STAGE = 2u * TILE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     const uint32_t slot_floats = slot_rows * (D + 2u);
@@ -137,12 +136,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             }
             if (lane == 0) {
                 mbar_arrive_expect_tx(bar, STAGE);
-                const int tok = (int)(pos % a.page_size);
-#pragma unroll
-                for (uint32_t h = 0; h < NH; ++h) {
-                    tma_page(st + h * HB, &kmap, (int)(64u * h), tok, (int)ci.kvh, page, bar);
-                    tma_page(st + TILE + h * HB, &vmap, (int)(64u * h), tok, (int)ci.kvh, page, bar);
-                }
+                const int part = (int)(ci.kvh * heads.part0);
+                const int group = (int)(ci.kvh * heads.group0 + pos % a.page_size / 8u);
+                tma_page(st, &kmap, part, group, page, bar);
+                tma_page(st + TILE, &vmap, part, group, page, bar);
             }
             si = si + 1u == stages ? 0u : si + 1u;
             ++issued;
@@ -183,7 +180,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 #pragma unroll
                 for (int nt = 0; nt < D / 8; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
             }
-            if (!mbar_wait(&bars[warp][s_cons], parity, err)) {
+            if (!quick_wait(&bars[warp][s_cons], parity, err)) {
                 ok = false;
                 break;
             }
@@ -198,7 +195,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
                 for (int kk = 0; kk < D / 16; kk += 2) {
                     uint32_t b[4];
                     const uint32_t ch = 2u * (kk & 3) + mi;  // 16-byte column of the 128-byte row
-                    ldmatrix4(b, ks + (kk >> 2) * HB + (8u * pb + mr) * 128u + ((ch ^ mr) << 4));
+                    ldmatrix4(b, ks + pb * GB + (kk >> 2) * 1024u + mr * 128u + ((ch ^ mr) << 4));
                     mma_16816<BF16>(sc[pb], qa[kk], b[0], b[1]);
                     mma_16816<BF16>(sc[pb], qa[kk + 1], b[2], b[3]);
                 }
@@ -254,7 +251,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             for (int nt = 0; nt < D / 8; nt += 2) {
                 uint32_t v[4];
                 const uint32_t ch = (nt & 7) + (mi >> 1);
-                ldmatrix4_trans(v, vs + (nt >> 3) * HB + (8u * (mi & 1u) + mr) * 128u + ((ch ^ mr) << 4));
+                ldmatrix4_trans(v, vs + (mi & 1u) * GB + (nt >> 3) * 1024u + mr * 128u + ((ch ^ mr) << 4));
                 mma_16816<BF16>(o[nt], pa, v[0] & keep[0], v[1] & keep[1]);
                 mma_16816<BF16>(o[nt + 1], pa, v[2] & keep[0], v[3] & keep[1]);
             }
@@ -440,8 +437,8 @@ int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args&
     cudaError_t e = cudaSuccess;
     if (few) {
         CUtensorMap kmap, vmap;
-        int st = encode_pages(&kmap, kv, kv.k_pages, kRowTile);
-        if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, kRowTile);
+        PageMap heads;
+        const int st = encode_pages(&kmap, &vmap, &heads, kv, kRowTile);
         if (st != ARC_OK) return st;
         const uint32_t slot_rows = !many && a.max_new * a.gq <= 8u ? 8u : 16u;
         const uint32_t fixed = 1024u + kRowWarps * slot_rows * (D + 2u) * 4u + 4u * (a.n_requests + 1u);
@@ -450,7 +447,7 @@ int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args&
                                  (int)kMost);
         if (e == cudaSuccess)
             e = launch_kernel(attn_paged_rows_kernel<D, BF16>, dim3(kSms), dim3(kRowWarps * 32u),
-                              fixed + kRowWarps * stages * kStage, stream, kmap, vmap, a, slot_rows, stages, recs,
+                              fixed + kRowWarps * stages * kStage, stream, kmap, vmap, heads, a, slot_rows, stages, recs,
                               parts, dev_error_word());
     }
     if (e == cudaSuccess && many) {
@@ -466,17 +463,26 @@ int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args&
 
 }  // namespace
 
-int paged::encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens) {
+int paged::encode_pages(CUtensorMap* k, CUtensorMap* v, PageMap* heads, const arcllm_cuda_paged_kv& kv,
+                        uint32_t tokens) {
     const EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return set_error(ARC_E_CUDA, "attention paged: cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[4] = {kv.head_dim, kv.page_size, kv.kv_heads, kv.n_pages};
-    const cuuint64_t strides[3] = {2ull * kv.token_stride, 2ull * kv.head_stride, 2ull * kv.page_stride};
-    const cuuint32_t box[4] = {64, tokens, 1, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult rc =
-        fn(map, kv.type == ARC_GGML_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-           const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return rc == CUDA_SUCCESS ? ARC_OK : set_error(ARC_E_CUDA, "attention paged: tensor map of the pages");
+    const cuuint32_t parts = kv.head_dim / 64u, groups = kv.page_size / 8u;
+    const bool by_token = kv.kv_heads == 1u || kv.head_stride == kv.head_dim;
+    *heads = by_token ? PageMap{parts, 0u} : PageMap{0u, groups};
+    const cuuint64_t dims[5] = {64, 8, by_token ? (cuuint64_t)kv.kv_heads * parts : parts,
+                                by_token ? groups : (cuuint64_t)kv.kv_heads * groups, kv.n_pages};
+    const cuuint64_t strides[4] = {2ull * kv.token_stride, 128, 16ull * kv.token_stride, 2ull * kv.page_stride};
+    const cuuint32_t box[5] = {64, 8, parts, tokens / 8u, 1}, one[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < 2; ++i) {
+        const CUresult rc =
+            fn(i ? v : k,
+               kv.type == ARC_GGML_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+               i ? kv.v_pages : kv.k_pages, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (rc != CUDA_SUCCESS) return set_error(ARC_E_CUDA, "attention paged: tensor map of the pages");
+    }
+    return ARC_OK;
 }
 
 int attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint64_t* out) {
@@ -512,8 +518,10 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
     if (off16(p.q) || off16(p.out) || off16(kv.k_pages) || off16(kv.v_pages) || off16(p.workspace) ||
         p.q_stride % 8u || p.out_stride % 8u || kv.page_stride % 8u || kv.token_stride % 8u || kv.head_stride % 8u)
         return set_error(ARC_E_ALIGNMENT, "attention paged: pointers and strides of 16 bytes");
-    if (kv.page_stride >= (1ull << 39) )
-        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: page stride past 2^40 bytes");
+    if (kv.kv_heads > 1u && kv.head_stride != kv.head_dim && kv.head_stride != (uint64_t)kv.page_size * kv.token_stride)
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: heads side by side in a token, or one after another");
+    if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31))
+        return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: a stride past 2^40 bytes");
     if (p.workspace_bytes < need) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: workspace too small");
     Args a{};
     a.q = static_cast<const uint16_t*>(p.q);

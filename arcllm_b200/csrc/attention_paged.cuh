@@ -78,6 +78,14 @@ struct Record {
     uint32_t valid, last_cta, row0, rows, kvh, pad[3];
 };
 
+// mbar_wait whose first tries do not read the global timer: the read takes longer
+// than most of these waits do, and what arrives meanwhile is seen after it.
+__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, unsigned int* err) {
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, err);
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -144,18 +152,28 @@ __device__ __forceinline__ uint32_t scan_units(const Args& a, uint32_t* off, uns
     return too_many ? 0u : (uint32_t)base;
 }
 
-// Box of the pages' tensor (dim, token, KV head, page) into shared memory; out of range reads zero.
-__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int dim, int token, int head, int page,
+// The pages as a tensor of (64 dims, 8 tokens, 64-dim parts, groups of 8 tokens,
+// pages): a box of all parts of some groups of one page arrives in shared memory
+// as [group][part][8 tokens][128 bytes], one copy for what would be a copy per
+// part otherwise (a copy costs about 50 clocks beside its 2.2 per 128 bytes:
+// 32 KB in boxes of 16 tokens 1390 -> 963 clocks).  KV heads are a stretch of the
+// parts where pages hold token after token, of the groups where they hold head
+// after head.
+struct PageMap {
+    uint32_t part0, group0;  // what one KV head adds to the coordinates
+};
+// Out of range (a page number of none) reads zeros.
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int part, int group, int page,
                                          uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4, "
         "%5}], [%6];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(token), "r"(head), "r"(page), "r"(smem_addr(bar))
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(part), "r"(group), "r"(page), "r"(smem_addr(bar))
         : "memory");
 }
 
-// Tensor map of K or V: boxes of `tokens` positions x 64 dims of one head of one page, 128-byte swizzle.
-int encode_pages(CUtensorMap* map, const arcllm_cuda_paged_kv& kv, const void* base, uint32_t tokens);
+// Tensor maps of K and V with boxes of `tokens` positions of one head of one page, 128-byte swizzle.
+int encode_pages(CUtensorMap* k, CUtensorMap* v, PageMap* heads, const arcllm_cuda_paged_kv& kv, uint32_t tokens);
 
 // The requests with more than kRowMax packed rows (attention_paged_tiles.cu).
 template <int D, bool BF16>

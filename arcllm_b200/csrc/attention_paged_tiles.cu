@@ -39,8 +39,9 @@ constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that is l
 
 template <int D>
 struct Layout {
-    static constexpr uint32_t kHalves = D / 64;               // 64-dim columns of 128 rows x 128 bytes
-    static constexpr uint32_t kBytes = kHalves * 16384u;      // a Q half, a K tile or a V tile
+    static constexpr uint32_t kParts = D / 64;           // 64-dim parts: a row of one is 128 bytes
+    static constexpr uint32_t kGroup = kParts * 1024u;   // 8 rows: [part][8][128 bytes], as the pages' boxes arrive
+    static constexpr uint32_t kBytes = 16u * kGroup;     // a Q half, a K tile or a V tile: 128 rows
     static constexpr uint32_t kStages = 4u * 128u / D;        // K and V tiles in the ring: 128 KB
     static constexpr uint32_t kRing = 2u * kBytes;            // after the two Q halves
     static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
@@ -70,6 +71,10 @@ struct Walk {
     __device__ __forceinline__ bool next(const Args& a, const uint32_t* off, uint32_t per_item) {
         left -= end() - i;
         if (left == 0) return false;
+        step(a, off, per_item);
+        return true;
+    }
+    __device__ __forceinline__ void step(const Args& a, const uint32_t* off, uint32_t per_item) {
         i = 0;
         if (++mt == n_items) {
             mt = 0;
@@ -82,7 +87,6 @@ struct Walk {
             }
         }
         item(a, per_item);
-        return true;
     }
 };
 
@@ -93,19 +97,77 @@ __device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint
 
 // A role's wait: false once any role has given up.  The same for all lanes.
 __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-    const bool here = mbar_wait(bar, parity, err) && !*abort_flag;
+    bool here = false;
+    for (int i = 0; i < 64 && !here; ++i) here = mbar_try_wait(bar, parity);
+    if (!here) here = !*abort_flag && mbar_wait(bar, parity, err);
     return __all_sync(0xffffffffu, here);
 }
 
-// Positions at, of a tile, that some row of the item sees (lo, hi its positions).
-__device__ __forceinline__ bool any_sees(const Args& a, uint32_t lo, uint32_t hi, uint32_t at) {
-    return at <= hi && (a.window == 0u || at + a.window > lo || at < a.sinks);
+// ---- packed pairs of fp32 ------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// largest of the values, NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^y of a pair without the exponential unit (16 results per clock and SM, the
+// bound of this kernel's softmax): y = n + f with n the nearest integer (adding
+// 1.5 2^23 leaves it in the low mantissa bits), |f| <= 1/2, a polynomial for 2^f
+// (least relative error over +-1/2: degree 3 7.5e-5 = 2^-13.7 for bf16 weights,
+// degree 4 2.6e-6 = 2^-18.5 for fp16 ones) and n added to the exponent.  y below
+// -126 counts as -126.
+template <bool BF16>
+__device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
+    const float2 y = unpair(y2);
+    y2 = pair(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
+    const uint64_t t = add2(y2, pair(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), y2);
+    uint64_t p;
+    if constexpr (BF16) {
+        p = fma2(f, pair(0.0551716527f, 0.0551716527f), pair(0.242611121f, 0.242611121f));
+        p = fma2(p, f, pair(0.693260988f, 0.693260988f));
+        p = fma2(p, f, pair(0.999928074f, 0.999928074f));
+    } else {
+        p = fma2(f, pair(0.00957010002f, 0.00957010002f), pair(0.0559178602f, 0.0559178602f));
+        p = fma2(p, f, pair(0.240247449f, 0.240247449f));
+        p = fma2(p, f, pair(0.693121815f, 0.693121815f));
+        p = fma2(p, f, pair(0.999999261f, 0.999999261f));
+    }
+    const float2 q = unpair(p), n = unpair(t);
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
 }
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, Args a,
-                            uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
+    attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                            PageMap heads, Args a, uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
                             unsigned int* err) {
     using L = Layout<D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -205,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
     Walk w;
     if (n_units != 0) {
@@ -222,36 +284,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t boxes = kTile / box;
         uint32_t stage = 0, phase = 0, issued = 0;
         bool bad_page = false, ok = true;
-        do {
-            for (uint32_t i = w.i; i < w.end() && ok; ++i) {
-                const uint32_t p = w.s.tile(i) * kTile + lane * box;  // lane b: box b of the tile
-                bool need = false;
-                int page = 0;
-                if (lane < boxes) {  // a box is loaded when it holds anything seen
-                    const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
-                    need = p <= w.hi && (p + box > from || p < a.sinks);
-                    if (need) page = a.table[(uint64_t)w.r * a.table_stride + p / a.page_size];
-                    if ((uint32_t)page >= a.n_pages) bad_page = true, page = (int)a.n_pages;  // reads zeros
-                }
-                const uint32_t n_need = __popc(__ballot_sync(0xffffffffu, need));
+        // lane b: box b of a tile; it is loaded when it holds anything that is seen
+        auto entry = [&](const Walk& x) -> int {
+            const uint32_t p = x.s.tile(x.i) * kTile + lane * box;
+            const uint32_t from = a.window && x.lo >= a.window ? x.lo - a.window + 1u : 0u;
+            if (lane >= boxes || p > x.hi || (p + box <= from && p >= a.sinks)) return -1;
+            const int page = a.table[(uint64_t)x.r * a.table_stride + p / a.page_size];
+            if ((uint32_t)page < a.n_pages) return page;
+            bad_page = true;
+            return (int)a.n_pages;  // reads zeros
+        };
+        int page = entry(w);
+        for (bool more = true; ok && more;) {
+            const uint32_t kvh = w.kvh, token = (w.s.tile(w.i) * kTile + lane * box) % a.page_size;
+            const int now = page;
+            ++w.i;
+            if (w.left-- == 1u)
+                more = false;
+            else if (w.i == w.s.n)
+                w.step(a, off, per_item);
+            if (more) page = entry(w);  // while this tile waits for its places
+            const uint32_t n_need = __popc(__ballot_sync(0xffffffffu, now >= 0));
+            const int part = (int)(kvh * heads.part0), group = (int)(kvh * heads.group0 + token / 8u);
 #pragma unroll
-                for (uint32_t kv = 0; kv < 2; ++kv) {
-                    if (issued >= L::kStages) ok = role_wait(&kv_empty[stage], phase ^ 1u, &abort_flag, err);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], n_need * L::kHalves * box * 128u);
-                    __syncwarp();
-                    if (need) {
-                        uint8_t* dst = smem + L::kRing + stage * L::kBytes + lane * box * 128u;
-#pragma unroll
-                        for (uint32_t h = 0; h < L::kHalves; ++h)
-                            tma_page(dst + h * 16384u, kv ? &vmap : &kmap, (int)(64u * h), (int)(p % a.page_size),
-                                     (int)w.kvh, page, &kv_full[stage]);
-                    }
-                    ++issued;
-                    if (++stage == L::kStages) stage = 0, phase ^= 1u;
-                }
+            for (uint32_t kv = 0; kv < 2; ++kv) {
+                if (issued >= L::kStages) ok = role_wait(&kv_empty[stage], phase ^ 1u, &abort_flag, err);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], n_need * (box / 8u) * L::kGroup);
+                __syncwarp();
+                if (now >= 0)
+                    tma_page(smem + L::kRing + stage * L::kBytes + lane * (box / 8u) * L::kGroup, kv ? &vmap : &kmap,
+                             part, group, now, &kv_full[stage]);
+                ++issued;
+                if (++stage == L::kStages) stage = 0, phase ^= 1u;
             }
-        } while (ok && w.next(a, off, per_item));
+        }
         if (!ok) {  // no copy may still be landing at the end
             abort_flag = 1;
             for (uint32_t k = issued > L::kStages ? issued - L::kStages : 0u; k < issued; ++k)
@@ -265,14 +332,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t stage = 0, phase = 0, n_item[2] = {0, 0}, n_s[2] = {0, 0};
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = role_wait(bar, parity, &abort_flag, err); };
+        const uint32_t leader = lane == 0;
         auto qk = [&](uint32_t s, uint32_t k_stage) {
-            const uint64_t qa = operand_desc(qs + s * L::kBytes, 16u), kb = operand_desc(ring + k_stage * L::kBytes, 16u);
+            const uint64_t qa = operand_desc(qs + s * L::kBytes, 16u, L::kGroup),
+                           kb = operand_desc(ring + k_stage * L::kBytes, 16u, L::kGroup);
 #pragma unroll
             for (uint32_t kk = 0; kk < D / 16u; ++kk) {
-                const uint32_t o = ((kk >> 2) * 16384u + (kk & 3u) * 32u) >> 4;  // addresses count 16 bytes
-                mma_smem(tmem + s * 128u, qa + o, kb + o, kQk, kk != 0u);
+                const uint32_t o = ((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4;  // addresses count 16 bytes
+                mma_smem(tmem + s * 128u, qa + o, kb + o, kQk, kk != 0u, leader);
             }
-            mma_commit(&s_full[s]);
+            mma_commit(&s_full[s], leader);
         };
 #pragma unroll 1
         do {
@@ -285,30 +354,33 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                 if (!wait(&q_full[s], n_item[s] & 1u)) break;
                 ++n_item[s];
                 tmem_fence_after();
-                if (lane == 0) qk(s, stage);
+                qk(s, stage);
             }
             if (!ok) break;
-            if (lane == 0) mma_commit(&kv_empty[stage]);
+            mma_commit(&kv_empty[stage], leader);
             if (++stage == L::kStages) stage = 0, phase ^= 1u;
             for (uint32_t i = i0; i < i1 && ok; ++i) {
                 const uint32_t v_stage = stage;
-                const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 16384u);
+                const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 1024u, L::kGroup);
                 if (!wait(&kv_full[v_stage], phase)) break;
                 if (++stage == L::kStages) stage = 0, phase ^= 1u;
                 // V rows of positions that no row of the item sees are zeroed: what lies there may be anything,
                 // and the weight 0 does not stop a NaN.
                 const uint32_t p0 = w.s.tile(i) * kTile;
                 const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
-                if (p0 + kTile - 1u > w.hi || (p0 < from && p0 + kTile > a.sinks)) {
-#pragma unroll 1
-                    for (uint32_t r = 0; r < kTile; r += 4u) {  // 8 lanes a row of 128 bytes
-                        const uint32_t row = r + (lane >> 3);
-                        if (!any_sees(a, w.lo, w.hi, p0 + row))
+                const bool tail = p0 + kTile - 1u > w.hi, gap = p0 < from && p0 + kTile > a.sinks;
+                if (tail || gap) {
+                    uint8_t* v = smem + L::kRing + v_stage * L::kBytes + (lane & 7u) * 16u;
+                    auto clear = [&](uint32_t r0, uint32_t r1) {  // rows [r0, r1): 8 lanes a row of 128 bytes
+#pragma unroll 2
+                        for (uint32_t r = r0 + (lane >> 3); r < r1; r += 4u)
 #pragma unroll
-                            for (uint32_t h = 0; h < L::kHalves; ++h)
-                                *reinterpret_cast<uint4*>(smem + L::kRing + v_stage * L::kBytes + h * 16384u +
-                                                          row * 128u + (lane & 7u) * 16u) = make_uint4(0, 0, 0, 0);
-                    }
+                            for (uint32_t c = 0; c < L::kParts; ++c)
+                                *reinterpret_cast<uint4*>(v + (r >> 3) * L::kGroup + c * 1024u + (r & 7u) * 128u) =
+                                    make_uint4(0, 0, 0, 0);
+                    };
+                    if (gap) clear(max(a.sinks, p0) - p0, min(from - p0, kTile));
+                    if (tail) clear(w.hi + 1u - p0, kTile);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
@@ -319,28 +391,24 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                     if (!wait(&p_full[s], n_s[s] & 1u)) break;
                     ++n_s[s];
                     tmem_fence_after();
-                    if (lane == 0) {
 #pragma unroll
-                        for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
-                            mma_tmem(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u,
-                                     vb + kk * (2048u >> 4), kPv, i != i0 || kk != 0u);
-                        if (s + 1u == subs) mma_commit(&kv_empty[v_stage]);
-                    }
+                    for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
+                        mma_tmem(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv,
+                                 i != i0 || kk != 0u, leader);
+                    if (s + 1u == subs) mma_commit(&kv_empty[v_stage], leader);
                     if (more) {
                         if (s == 0 && !wait(&kv_full[stage], phase)) break;
-                        if (lane == 0) {
-                            qk(s, stage);
-                            if (s + 1u == subs) mma_commit(&kv_empty[stage]);
-                        }
-                    } else if (lane == 0) {
-                        mma_commit(&o_full[s]);
+                        qk(s, stage);
+                        if (s + 1u == subs) mma_commit(&kv_empty[stage], leader);
+                    } else {
+                        mma_commit(&o_full[s], leader);
                     }
                 }
                 if (more && ok && ++stage == L::kStages) stage = 0, phase ^= 1u;
             }
         } while (ok && w.next(a, off, per_item));
         if (!ok) abort_flag = 1;
-        if (lane == 0) mma_commit(&done);
+        mma_commit(&done, leader);
         __syncwarp();
         mbar_wait(&done, 0, err);  // nothing of this CTA runs on the tensor core any more
       }
@@ -351,57 +419,82 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
         const uint32_t s = warp >> 2, t = tid & 127u;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t ts = tmem + lanes + s * 128u, to = tmem + lanes + 256u + s * 128u;
-        uint8_t* qdst = smem + s * L::kBytes + (t >> 3) * 1024u + (t & 7u) * 128u;
         uint32_t n_s = 0, n_o = 0, u = U0;
+        const uint32_t t_row = t / a.gq, t_head = t - t_row * a.gq;
+        // Row t of Q, when the half has rows in the item; its place is free once S of the item before is there.
+        auto load_q = [&](const Walk& x) {
+            if (s * half_rows >= x.rows) return;
+            const bool live = t_row < min(half_rows, x.rows - s * half_rows);
+            const uint4* src = reinterpret_cast<const uint4*>(
+                a.q + (uint64_t)(x.q.row0 + x.first + s * half_rows + (live ? t_row : 0u)) * a.q_stride +
+                (x.kvh * a.gq + t_head) * D);
+            uint8_t* dst = smem + s * L::kBytes + (t >> 3) * L::kGroup + (t & 7u) * 128u;
+#pragma unroll
+            for (uint32_t c = 0; c < D / 8u; ++c) {
+                const uint4 v = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * 1024u + (((c & 7u) ^ (t & 7u)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[s]);
+        };
+        load_q(w);
         bool ok = true;
-        do {
+        for (bool more = true; more;) {
             const uint32_t i0 = w.i, i1 = w.end(), item_u0 = u - i0;
             u += i1 - i0;
-            if (s * half_rows >= w.rows) continue;  // this half has no rows (uniform over its warps)
-            const uint32_t sub_rows = min(half_rows, w.rows - s * half_rows), packed = sub_rows * a.gq;
-            const uint32_t qr = min(t / a.gq, sub_rows - 1u);
-            const uint32_t pos = w.lo + s * half_rows + qr;
-            const uint64_t row = w.q.row0 + w.first + s * half_rows + qr;
-            const uint32_t col = (w.kvh * a.gq + t % a.gq) * D;
-            {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.q_stride + col);
-#pragma unroll
-                for (uint32_t c = 0; c < D / 8u; ++c) {
-                    const uint4 v = t < packed ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(qdst + (c >> 3) * 16384u + (((c & 7u) ^ (t & 7u)) << 4)) = v;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tmem_fence_before();  // the last item's O has been read
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[s]);
+            Walk nw = w;
+            if (s * half_rows >= w.rows) {  // this half has no rows (uniform over its warps)
+                more = nw.next(a, off, per_item);
+                if (more) load_q(nw);
+                w = nw;
+                continue;
             }
+            const uint32_t sub_rows = min(half_rows, w.rows - s * half_rows);
             const uint32_t p_lo = w.lo + s * half_rows, p_hi = p_lo + sub_rows - 1u;
+            const uint32_t pos = p_lo + min(t_row, sub_rows - 1u);
             float m = -INFINITY, l = 0.f;
             for (uint32_t i = i0; i < i1; ++i) {
                 ok = role_wait(&s_full[s], n_s & 1u, &abort_flag, err);
                 if (!ok) break;
                 ++n_s;
                 tmem_fence_after();
-                float x[4][32];
-#pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) tmem_ld32(ts + 32u * k, x[k]);
                 const uint32_t p0 = w.s.tile(i) * kTile;
-                if (p0 + kTile - 1u > p_lo ||
-                    (a.window && p0 + a.window <= p_hi && p0 + kTile > a.sinks)) {  // not all rows see all of it
+                // not all rows see all of it: behind a row's position, before its window and past the sinks
+                const bool past = p0 + kTile - 1u > p_lo;
+                const bool before = a.window && p0 + a.window <= p_hi && p0 + kTile > a.sinks;
+                const int last = (int)(pos - p0);
+                int first = 0, sinks = 0;
+                if (before && pos + 1u >= a.window) first = (int)(pos + 1u - a.window - p0), sinks = (int)(a.sinks - p0);
+                // 32 columns at a time in a loop that stays one: tensor memory gives 128 columns in 90 clocks, so S is
+                // read twice rather than kept in 128 registers, and the code of all roles stays small enough for the
+                // instruction caches, which straight-line code for 128 columns was not.
+                auto columns = [&](uint32_t c0, float (&x)[32]) {
+                    tmem_ld32(ts + c0, x);
+                    if (past || before) {
+                        const int e = last - (int)c0, f = first - (int)c0, g = sinks - (int)c0;
 #pragma unroll
-                    for (uint32_t c = 0; c < 128u; ++c)
-                        if (!visible(a, pos, p0 + c)) x[c / 32u][c % 32u] = -INFINITY;
+                        for (int c = 0; c < 32; ++c)
+                            if (c > e || (c < f && c >= g)) x[c] = -INFINITY;
+                    }
+                };
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+                for (uint32_t c0 = 0; c0 < kTile; c0 += 32u) {
+                    float x[32];
+                    columns(c0, x);
+#pragma unroll
+                    for (uint32_t c = 0; c < 32u; c += 4u)
+#pragma unroll
+                        for (uint32_t k = 0; k < 2u; ++k) mx[k] = max_nan(mx[k], x[c + 2u * k], x[c + 2u * k + 1u]);
                 }
-                float mx[4] = {x[0][0], x[1][0], x[2][0], x[3][0]};
-#pragma unroll
-                for (uint32_t c = 1; c < 32u; ++c)
-#pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) mx[k] = fmaxf(mx[k], x[k][c]);
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+                // An infinite score has no softmax: NaN for the row, as for a NaN score.
+                float mn = max_nan(mx[0], mx[1]) * a.scale_log2;
+                if (mn == INFINITY) mn = NAN;
                 if (i == i0) {
                     m = mn;  // O is written afresh
-                } else if (__any_sync(0xffffffffu, mn > m + kGrow)) {
-                    const float to_m = fmaxf(m, mn);
+                } else if (__any_sync(0xffffffffu, !(mn <= m + kGrow))) {
+                    const float to_m = max_nan(m, mn);
                     const float f = ex2(m - (to_m == -INFINITY ? 0.f : to_m));
                     l *= f;
                     m = to_m;
@@ -416,48 +509,66 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+                for (uint32_t c0 = 0; c0 < kTile; c0 += 32u) {
+                    float x[32];
+                    columns(c0, x);
+                    uint32_t pk[16];
 #pragma unroll
-                for (uint32_t c0 = 0; c0 < 128u; c0 += 64u) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (uint32_t c = 0; c < 64u; c += 2u) {
-                        const float e0 = ex2(fmaf(x[(c0 + c) / 32u][c % 32u], a.scale_log2, -ref));
-                        const float e1 = ex2(fmaf(x[(c0 + c) / 32u][c % 32u + 1u], a.scale_log2, -ref));
-                        sum[c & 2u] += e0, sum[(c & 2u) + 1u] += e1;
+                    for (uint32_t c = 0; c < 32u; c += 2u) {
+                        const uint64_t y2 = fma2(pair(x[c], x[c + 1u]), c2, r2);
+                        float2 e;
+                        if (c % 8u == 6u) {
+                            e = exp2_poly<BF16>(y2);
+                        } else {
+                            const float2 y = unpair(y2);
+                            e = make_float2(ex2(y.x), ex2(y.y));
+                        }
+                        sum[(c >> 1) & 1u] = add2(sum[(c >> 1) & 1u], pair(e.x, e.y));
                         // the product takes weights of the cache's type: half a step of it each, as the output
-                        pk[c / 2u] = pack16<BF16>(e0, e1);
+                        pk[c / 2u] = pack16<BF16>(e.x, e.y);
                     }
-                    tmem_st32(ts + c0 / 2u, pk);
+                    tmem_st16(ts + c0 / 2u, pk);  // over columns that have been read
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 sm = unpair(add2(sum[0], sum[1]));
+                l += sm.x + sm.y;
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[s]);
             }
-            if (ok) ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
+            // The next item's Q goes in while the last product runs; its S may follow at once, its O only after
+            // this thread has handed over weights, and by then it has read O.
+            if (ok) {
+                more = nw.next(a, off, per_item);
+                if (more) load_q(nw);
+                ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
+            }
             if (!ok) break;
             ++n_o;
             tmem_fence_after();
-            const bool whole = i0 == 0 && i1 == w.s.n;
+            const bool whole = i0 == 0 && i1 == w.s.n, live = t_row < sub_rows;
             const uint32_t slot = i0 != 0 ? 0u : 1u;  // began before this stretch, or goes on after it
             float* part = parts + (uint64_t)(blockIdx.x * 2u + slot) * (kTileRows * (D + 2u));
             const uint32_t ri = s * half_rows * a.gq + t;
+            uint16_t* out = a.out + (uint64_t)(w.q.row0 + w.first + s * half_rows + t_row) * a.out_stride +
+                            (w.kvh * a.gq + t_head) * D;
             const float inv = 1.f / l;
 #pragma unroll 1
             for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
                 float o[32];
                 tmem_ld32(to + c, o);
-                if (t < packed && whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + col + c);
+                if (live && whole) {
+                    uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
                     for (uint32_t k = 0; k < 4u; ++k)
                         dst[k] = make_uint4(pack16<BF16>(o[8 * k] * inv, o[8 * k + 1] * inv),
                                             pack16<BF16>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
                                             pack16<BF16>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
                                             pack16<BF16>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
-                } else if (t < packed) {
+                } else if (live) {
                     float4* dst = reinterpret_cast<float4*>(part + (uint64_t)ri * D + c);
 #pragma unroll
                     for (uint32_t k = 0; k < 8u; ++k)
@@ -465,13 +576,15 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                 }
                 __syncwarp();
             }
+            tmem_fence_before();  // O has been read
             if (!whole) {
-                if (t < packed) *reinterpret_cast<float2*>(part + kTileRows * D + 2u * ri) = make_float2(m, l);
+                if (live) *reinterpret_cast<float2*>(part + kTileRows * D + 2u * ri) = make_float2(m, l);
                 if (slot == 1u && tid == 0)
                     recs[blockIdx.x] = {1u, (item_u0 + w.s.n - 1u) / per, w.q.row0 + w.first, w.rows * a.gq, w.kvh,
                                         {0, 0, 0}};
             }
-        } while (w.next(a, off, per_item));
+            w = nw;
+        }
         if (!ok) abort_flag = 1;
       }
     }
@@ -488,15 +601,15 @@ int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, fl
     uint32_t box = 16;  // the largest power of two up to the tile that divides the page
     while (box < kTile && kv.page_size % (2u * box) == 0u) box *= 2u;
     CUtensorMap kmap, vmap;
-    int st = encode_pages(&kmap, kv, kv.k_pages, box);
-    if (st == ARC_OK) st = encode_pages(&vmap, kv, kv.v_pages, box);
+    PageMap heads;
+    const int st = encode_pages(&kmap, &vmap, &heads, kv, box);
     if (st != ARC_OK) return st;
     const uint32_t smem = 1024u + L::kOff + 4u * (a.n_requests + 1u);
     cudaError_t e = cudaFuncSetAttribute(attn_paged_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
     if (e == cudaSuccess)
-        e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap, a,
-                          box, 1u, recs, parts, dev_error_word());
+        e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap,
+                          heads, a, box, 1u, recs, parts, dev_error_word());
     return e == cudaSuccess ? ARC_OK : set_cuda_error(e, "attention paged tiles launch");
 }
 

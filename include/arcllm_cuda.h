@@ -479,8 +479,10 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  *   scale        on q.k, > 0 (1/sqrt(head_dim) unless the model says otherwise);
  *   workspace    arcllm_cuda_attention_paged_workspace bytes, any content;
  *                calls that may overlap in time need one each.
- * head_dim 64 or 128, q_heads/kv_heads 1..16, page_size a multiple of 16,
- * n_requests <= 4096; pointers 16-byte aligned, strides multiples of 8.
+ * head_dim 64 or 128, q_heads/kv_heads 1..128, page_size a multiple of 16,
+ * n_requests <= 4096; pointers 16-byte aligned, strides multiples of 8; the
+ * heads of a page side by side in each token (head_stride = head_dim) or one
+ * after another (head_stride = page_size * token_stride).
  * A request whose lengths do not fit (kv_total < n, n > max_new, a table row
  * too short, rows past max_rows) is skipped and sets the bounds bit; a page
  * number outside [0, n_pages) sets it too and reads as zeros. */
