@@ -58,6 +58,10 @@ struct Walk {
     __device__ __forceinline__ void enter(const Args& a, uint32_t per_item) {
         bool bad = false;
         load_req(a, r, q, bad);
+        // the same for all lanes, and known to be
+        q.row0 = __shfl_sync(0xffffffffu, q.row0, 0);
+        q.n = __shfl_sync(0xffffffffu, q.n, 0);
+        q.p0 = __shfl_sync(0xffffffffu, q.p0, 0);
         n_items = (q.n + per_item - 1u) / per_item;
     }
     __device__ __forceinline__ void item(const Args& a, uint32_t per_item) {
@@ -95,12 +99,20 @@ __device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint
     return span_of<kTile>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
 }
 
-// A role's wait: false once any role has given up.  The same for all lanes.
+// A role's wait: false once any role has given up.  One vote decides for the
+// warp: a wait that is over costs 96 clocks this way, 215 with a branch of its
+// own for each lane (and the MMA warp waits six times per tile).
 __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-    bool here = false;
-    for (int i = 0; i < 64 && !here; ++i) here = mbar_try_wait(bar, parity);
-    if (!here) here = !*abort_flag && mbar_wait(bar, parity, err);
-    return __all_sync(0xffffffffu, here);
+    unsigned long long t0 = 0;
+    for (uint32_t n = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++n) {
+        if (n < 64u) continue;  // the first tries do not read the timer
+        const unsigned long long t = globaltimer();
+        if (n == 64u) t0 = t;
+        const bool late = t - t0 > kWaitLimitNs;
+        if (late) raise_error(err, ARC_DEV_ERR_TIMEOUT);
+        if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
+    }
+    return true;
 }
 
 // ---- packed pairs of fp32 ------------------------------------------------------
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     if (tid == 0) {
         for (uint32_t s = 0; s < L::kStages; ++s) mbar_init(&kv_full[s], 1), mbar_init(&kv_empty[s], 1);
         for (uint32_t s = 0; s < 2; ++s) {
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     });
     const uint32_t per = max((total + gridDim.x - 1u) / gridDim.x, least);
     const uint32_t U0 = (uint32_t)min((unsigned long long)blockIdx.x * per, (unsigned long long)total);
-    const uint32_t n_units = min(per, total - U0);
+    const uint32_t n_units = __shfl_sync(0xffffffffu, min(per, total - U0), 0);
     if (tid == 0) recs[blockIdx.x].valid = 0;
     if (n_units != 0 && warp == 10) {
         const uint32_t r = request_of(off, a.n_requests, U0);
@@ -271,7 +283,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     Walk w;
     if (n_units != 0) {
-        w.r = start[0], w.kvh = start[1], w.mt = start[2], w.i = start[3], w.left = n_units;
+        w.r = __shfl_sync(0xffffffffu, start[0], 0), w.kvh = __shfl_sync(0xffffffffu, start[1], 0);
+        w.mt = __shfl_sync(0xffffffffu, start[2], 0), w.i = __shfl_sync(0xffffffffu, start[3], 0);
+        w.left = n_units;
         w.enter(a, per_item);
         w.item(a, per_item);
     }
