@@ -12,7 +12,10 @@
 // on the other's products.
 //   warps 0..3, 4..7  softmax of half 0, 1: also load Q, write the output
 //   warp 8            TMA: pages' K and V rows into a ring of tiles
-//   warp 9            issues the MMAs (10 and 11 only complete the warpgroup)
+//   warps 9, 10       issue the MMAs of half 0, 1 in turn: one waits for its
+//                     operands while the other issues, and the turn keeps the
+//                     halves out of step (without it both softmaxes ran at once
+//                     and then both products: 4500 clocks a unit)
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
 // last time (the sums carry the same factor, so the result is the same); MMAs
 // of one thread run in order, so when S of a tile is there, all products
@@ -185,20 +188,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
-    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], s_full[2], p_full[2], o_full[2], done;
+    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], s_full[2], p_full[2], o_full[2], turn[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     if (tid == 0) {
-        for (uint32_t s = 0; s < L::kStages; ++s) mbar_init(&kv_full[s], 1), mbar_init(&kv_empty[s], 1);
+        for (uint32_t s = 0; s < L::kStages; ++s) mbar_init(&kv_full[s], 1), mbar_init(&kv_empty[s], 2);
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(&q_full[s], 4);
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 4);
             mbar_init(&o_full[s], 1);
+            mbar_init(&turn[s], 1);
         }
-        mbar_init(&done, 1);
+        mbar_init(&done, 2);
         abort_flag = 0;
         fence_mbar_init();
     }
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t U0 = (uint32_t)min((unsigned long long)blockIdx.x * per, (unsigned long long)total);
     const uint32_t n_units = __shfl_sync(0xffffffffu, min(per, total - U0), 0);
     if (tid == 0) recs[blockIdx.x].valid = 0;
-    if (n_units != 0 && warp == 10) {
+    if (n_units != 0 && warp == 11) {
         const uint32_t r = request_of(off, a.n_requests, U0);
         Req q;
         bool bad = false;
@@ -339,47 +343,57 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_wait(&kv_full[k % L::kStages], (k / L::kStages) & 1u, err);
         }
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
-      } else if (warp == 9) {
-        // ---------------- MMA ----------------
+      } else if (warp < 11) {
+        // ---------------- MMA of half s ----------------
         constexpr uint32_t kQk = instr_desc<BF16>(128, false), kPv = instr_desc<BF16>(D, true);
-        const uint32_t ring = smem_addr(smem + L::kRing), qs = smem_addr(smem);
-        uint32_t stage = 0, phase = 0, n_item[2] = {0, 0}, n_s[2] = {0, 0};
+        const uint32_t s = warp - 9u, leader = lane == 0;
+        const uint32_t ring = smem_addr(smem + L::kRing), ts = tmem + s * 128u, to = tmem + 256u + s * 128u;
+        const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kBytes, 16u, L::kGroup);
+        uint32_t stage = 0, phase = 0, n_item = 0, n_p = 0, n_turn = s ^ 1u;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = role_wait(bar, parity, &abort_flag, err); };
-        const uint32_t leader = lane == 0;
-        auto qk = [&](uint32_t s, uint32_t k_stage) {
-            const uint64_t qa = operand_desc(qs + s * L::kBytes, 16u, L::kGroup),
-                           kb = operand_desc(ring + k_stage * L::kBytes, 16u, L::kGroup);
+        auto my_turn = [&]() {  // half 0 begins
+            const bool got = wait(&turn[s], n_turn++ & 1u);
+            tmem_fence_after();
+            return got;
+        };
+        auto pass_turn = [&]() {
+            if (leader) mbar_arrive(&turn[s ^ 1u]);
+        };
+        auto advance = [&]() {
+            if (++stage == L::kStages) stage = 0, phase ^= 1u;
+        };
+        auto qk = [&](uint32_t k_stage) {  // S = Q K^T
+            const uint64_t kb = operand_desc(ring + k_stage * L::kBytes, 16u, L::kGroup);
 #pragma unroll
             for (uint32_t kk = 0; kk < D / 16u; ++kk) {
                 const uint32_t o = ((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4;  // addresses count 16 bytes
-                mma_smem(tmem + s * 128u, qa + o, kb + o, kQk, kk != 0u, leader);
+                mma_smem(ts, qa + o, kb + o, kQk, kk != 0u, leader);
             }
             mma_commit(&s_full[s], leader);
         };
-#pragma unroll 1
         do {
-            const uint32_t i0 = w.i, i1 = w.end(), subs = w.rows > half_rows ? 2u : 1u;
-            // S of the first tile
+            const uint32_t i0 = w.i, i1 = w.end();
+            const bool live = s == 0u || w.rows > half_rows;  // otherwise the half only passes its turns on
             if (!wait(&kv_full[stage], phase)) break;
-            
-#pragma unroll 1
-for (uint32_t s = 0; s < subs && ok; ++s) {
-                if (!wait(&q_full[s], n_item[s] & 1u)) break;
-                ++n_item[s];
-                tmem_fence_after();
-                qk(s, stage);
-            }
-            if (!ok) break;
+            if (live && !wait(&q_full[s], n_item++ & 1u)) break;
+            if (!my_turn()) break;
+            if (live) qk(stage);
+            pass_turn();
             mma_commit(&kv_empty[stage], leader);
-            if (++stage == L::kStages) stage = 0, phase ^= 1u;
-            for (uint32_t i = i0; i < i1 && ok; ++i) {
+            advance();
+            for (uint32_t i = i0; i < i1; ++i) {
                 const uint32_t v_stage = stage;
-                const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 1024u, L::kGroup);
+                const bool more = i + 1u < i1;
                 if (!wait(&kv_full[v_stage], phase)) break;
-                if (++stage == L::kStages) stage = 0, phase ^= 1u;
-                // V rows of positions that no row of the item sees are zeroed: what lies there may be anything,
-                // and the weight 0 does not stop a NaN.
+                advance();
+                const uint32_t k_stage = stage;
+                if (more) {  // the next K too: nothing is waited for between the products
+                    if (!wait(&kv_full[k_stage], phase)) break;
+                    advance();
+                }
+                // V rows of positions that no row of the item sees are zeroed (by both warps): what lies there may be
+                // anything, and the weight 0 does not stop a NaN.
                 const uint32_t p0 = w.s.tile(i) * kTile;
                 const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
                 const bool tail = p0 + kTile - 1u > w.hi, gap = p0 < from && p0 + kTile > a.sinks;
@@ -398,27 +412,21 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                const bool more = i + 1u < i1;
-                
-#pragma unroll 1
-for (uint32_t s = 0; s < subs && ok; ++s) {
-                    if (!wait(&p_full[s], n_s[s] & 1u)) break;
-                    ++n_s[s];
-                    tmem_fence_after();
+                if (live && !wait(&p_full[s], n_p++ & 1u)) break;
+                if (!my_turn()) break;
+                if (live) {
+                    const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 1024u, L::kGroup);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
-                        mma_tmem(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv,
-                                 i != i0 || kk != 0u, leader);
-                    if (s + 1u == subs) mma_commit(&kv_empty[v_stage], leader);
-                    if (more) {
-                        if (s == 0 && !wait(&kv_full[stage], phase)) break;
-                        qk(s, stage);
-                        if (s + 1u == subs) mma_commit(&kv_empty[stage], leader);
-                    } else {
+                        mma_tmem(to, ts + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv, i != i0 || kk != 0u, leader);
+                    if (more)
+                        qk(k_stage);
+                    else
                         mma_commit(&o_full[s], leader);
-                    }
                 }
-                if (more && ok && ++stage == L::kStages) stage = 0, phase ^= 1u;
+                pass_turn();
+                mma_commit(&kv_empty[v_stage], leader);
+                if (more) mma_commit(&kv_empty[k_stage], leader);
             }
         } while (ok && w.next(a, off, per_item));
         if (!ok) abort_flag = 1;
@@ -480,25 +488,25 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                 const int last = (int)(pos - p0);
                 int first = 0, sinks = 0;
                 if (before && pos + 1u >= a.window) first = (int)(pos + 1u - a.window - p0), sinks = (int)(a.sinks - p0);
-                // 32 columns at a time in a loop that stays one: tensor memory gives 128 columns in 90 clocks, so S is
+                // 64 columns at a time in a loop that stays one: tensor memory gives 128 columns in 90 clocks, so S is
                 // read twice rather than kept in 128 registers, and the code of all roles stays small enough for the
                 // instruction caches, which straight-line code for 128 columns was not.
-                auto columns = [&](uint32_t c0, float (&x)[32]) {
-                    tmem_ld32(ts + c0, x);
+                auto columns = [&](uint32_t c0, float (&x)[64]) {
+                    tmem_ld64(ts + c0, x);
                     if (past || before) {
                         const int e = last - (int)c0, f = first - (int)c0, g = sinks - (int)c0;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
+                        for (int c = 0; c < 64; ++c)
                             if (c > e || (c < f && c >= g)) x[c] = -INFINITY;
                     }
                 };
                 float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                for (uint32_t c0 = 0; c0 < kTile; c0 += 32u) {
-                    float x[32];
+                for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
+                    float x[64];
                     columns(c0, x);
 #pragma unroll
-                    for (uint32_t c = 0; c < 32u; c += 4u)
+                    for (uint32_t c = 0; c < 64u; c += 4u)
 #pragma unroll
                         for (uint32_t k = 0; k < 2u; ++k) mx[k] = max_nan(mx[k], x[c + 2u * k], x[c + 2u * k + 1u]);
                 }
@@ -526,12 +534,12 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                 const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll 1
-                for (uint32_t c0 = 0; c0 < kTile; c0 += 32u) {
-                    float x[32];
+                for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
+                    float x[64];
                     columns(c0, x);
-                    uint32_t pk[16];
+                    uint32_t pk[32];
 #pragma unroll
-                    for (uint32_t c = 0; c < 32u; c += 2u) {
+                    for (uint32_t c = 0; c < 64u; c += 2u) {
                         const uint64_t y2 = fma2(pair(x[c], x[c + 1u]), c2, r2);
                         float2 e;
                         if (c % 8u == 6u) {
@@ -544,7 +552,7 @@ for (uint32_t s = 0; s < subs && ok; ++s) {
                         // the product takes weights of the cache's type: half a step of it each, as the output
                         pk[c / 2u] = pack16<BF16>(e.x, e.y);
                     }
-                    tmem_st16(ts + c0 / 2u, pk);  // over columns that have been read
+                    tmem_st32(ts + c0 / 2u, pk);  // over columns that have been read
                 }
                 const float2 sm = unpair(add2(sum[0], sum[1]));
                 l += sm.x + sm.y;
