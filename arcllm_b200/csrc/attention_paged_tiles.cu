@@ -50,10 +50,16 @@ struct Layout {
     static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
 };
 
-// The item that a role is at, and the part of its tiles that this CTA does.
+// An item costs about this many tiles beside its own (queries in, first S, last
+// product, output): they count when the CTAs' stretches are made equal, or one
+// that gets many short items takes half as long again.
+constexpr uint32_t kItemCost = 2;
+
+// The item that a role is at, and the part of its tiles that this CTA does: of
+// the item's units [0, kItemCost + tiles), from v on, as many as are left.
 struct Walk {
-    uint32_t r, kvh, mt, i, left;  // left: units of the CTA's stretch from here on
-    uint32_t n_items;              // of the request
+    uint32_t r, kvh, mt, v, left;
+    uint32_t n_items;  // of the request
     Req q;
     uint32_t first, rows;  // query rows [first, first + rows) of the request
     uint32_t lo, hi;       // their positions
@@ -74,32 +80,34 @@ struct Walk {
         hi = lo + rows - 1u;
         s = span_of<kTile>(a, lo, hi);
     }
-    __device__ __forceinline__ uint32_t end() const { return min(s.n, i + left); }
+    __device__ __forceinline__ uint32_t stop() const { return min(s.n + kItemCost, v + left); }
+    __device__ __forceinline__ uint32_t begin() const { return max(v, kItemCost) - kItemCost; }
+    __device__ __forceinline__ uint32_t end() const { return max(stop(), kItemCost) - kItemCost; }
+    // The next item with tiles for this CTA; false at the stretch's end.
     __device__ __forceinline__ bool next(const Args& a, const uint32_t* off, uint32_t per_item) {
-        left -= end() - i;
-        if (left == 0) return false;
-        step(a, off, per_item);
-        return true;
-    }
-    __device__ __forceinline__ void step(const Args& a, const uint32_t* off, uint32_t per_item) {
-        i = 0;
-        if (++mt == n_items) {
-            mt = 0;
-            if (++kvh == a.kv_heads) {
-                kvh = 0;
-                const uint32_t e = off[r + 1];
-                do ++r;
-                while (off[r + 1] == e);  // units are left, so a request with units follows
-                enter(a, per_item);
+        do {
+            left -= stop() - v;
+            if (left == 0) return false;
+            v = 0;
+            if (++mt == n_items) {
+                mt = 0;
+                if (++kvh == a.kv_heads) {
+                    kvh = 0;
+                    const uint32_t e = off[r + 1];
+                    do ++r;
+                    while (off[r + 1] == e);  // units are left, so a request with units follows
+                    enter(a, per_item);
+                }
             }
-        }
-        item(a, per_item);
+            item(a, per_item);
+        } while (begin() == end());
+        return true;
     }
 };
 
 __device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint32_t mt, uint32_t per_item) {
     const uint32_t first = mt * per_item, rows = min(per_item, q.n - first);
-    return span_of<kTile>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
+    return kItemCost + span_of<kTile>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
 }
 
 // A role's wait: false once any role has given up.  One vote decides for the
@@ -286,16 +294,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
     Walk w;
-    if (n_units != 0) {
+    bool any = n_units != 0;
+    if (any) {
         w.r = __shfl_sync(0xffffffffu, start[0], 0), w.kvh = __shfl_sync(0xffffffffu, start[1], 0);
-        w.mt = __shfl_sync(0xffffffffu, start[2], 0), w.i = __shfl_sync(0xffffffffu, start[3], 0);
+        w.mt = __shfl_sync(0xffffffffu, start[2], 0), w.v = __shfl_sync(0xffffffffu, start[3], 0);
         w.left = n_units;
         w.enter(a, per_item);
         w.item(a, per_item);
+        if (w.begin() == w.end()) any = w.next(a, off, per_item);
     }
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      if (n_units == 0) {
+      if (!any) {
         // nothing to do; the tensor memory is given back below
       } else if (warp == 8) {
         // ---------------- TMA: K, V, K, V ... tile by tile ----------------
@@ -303,8 +313,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t stage = 0, phase = 0, issued = 0;
         bool bad_page = false, ok = true;
         // lane b: box b of a tile; it is loaded when it holds anything that is seen
+        uint32_t i = w.begin(), end = w.end();
         auto entry = [&](const Walk& x) -> int {
-            const uint32_t p = x.s.tile(x.i) * kTile + lane * box;
+            const uint32_t p = x.s.tile(i) * kTile + lane * box;
             const uint32_t from = a.window && x.lo >= a.window ? x.lo - a.window + 1u : 0u;
             if (lane >= boxes || p > x.hi || (p + box <= from && p >= a.sinks)) return -1;
             const int page = a.table[(uint64_t)x.r * a.table_stride + p / a.page_size];
@@ -314,13 +325,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         int page = entry(w);
         for (bool more = true; ok && more;) {
-            const uint32_t kvh = w.kvh, token = (w.s.tile(w.i) * kTile + lane * box) % a.page_size;
+            const uint32_t kvh = w.kvh, token = (w.s.tile(i) * kTile + lane * box) % a.page_size;
             const int now = page;
-            ++w.i;
-            if (w.left-- == 1u)
-                more = false;
-            else if (w.i == w.s.n)
-                w.step(a, off, per_item);
+            if (++i == end) {
+                more = w.next(a, off, per_item);
+                i = w.begin(), end = w.end();
+            }
             if (more) page = entry(w);  // while this tile waits for its places
             const uint32_t n_need = __popc(__ballot_sync(0xffffffffu, now >= 0));
             const int part = (int)(kvh * heads.part0), group = (int)(kvh * heads.group0 + token / 8u);
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_commit(&s_full[s], leader);
         };
         do {
-            const uint32_t i0 = w.i, i1 = w.end();
+            const uint32_t i0 = w.begin(), i1 = w.end();
             const bool live = s == 0u || w.rows > half_rows;  // otherwise the half only passes its turns on
             if (!wait(&kv_full[stage], phase)) break;
             if (live && !wait(&q_full[s], n_item++ & 1u)) break;
@@ -436,12 +446,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-      if (n_units != 0) {
+      if (any) {
         // ---------------- softmax of half s: thread t has packed row t ----------------
         const uint32_t s = warp >> 2, t = tid & 127u;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t ts = tmem + lanes + s * 128u, to = tmem + lanes + 256u + s * 128u;
-        uint32_t n_s = 0, n_o = 0, u = U0;
+        uint32_t n_s = 0, n_o = 0;
         const uint32_t t_row = t / a.gq, t_head = t - t_row * a.gq;
         // Row t of Q, when the half has rows in the item; its place is free once S of the item before is there.
         auto load_q = [&](const Walk& x) {
@@ -463,8 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         load_q(w);
         bool ok = true;
         for (bool more = true; more;) {
-            const uint32_t i0 = w.i, i1 = w.end(), item_u0 = u - i0;
-            u += i1 - i0;
+            const uint32_t i0 = w.begin(), i1 = w.end();
             Walk nw = w;
             if (s * half_rows >= w.rows) {  // this half has no rows (uniform over its warps)
                 more = nw.next(a, off, per_item);
@@ -602,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!whole) {
                 if (live) *reinterpret_cast<float2*>(part + kTileRows * D + 2u * ri) = make_float2(m, l);
                 if (slot == 1u && tid == 0)
-                    recs[blockIdx.x] = {1u, (item_u0 + w.s.n - 1u) / per, w.q.row0 + w.first, w.rows * a.gq, w.kvh,
+                    recs[blockIdx.x] = {1u, (U0 + n_units - w.left - w.v + kItemCost + w.s.n - 1u) / per, w.q.row0 + w.first, w.rows * a.gq, w.kvh,
                                         {0, 0, 0}};
             }
             w = nw;
