@@ -10,12 +10,14 @@
 //   O_s += P_s V         tcgen05.mma, P in tensor memory, V in shared memory
 // The halves alternate: while one half's softmax runs, the tensor core works
 // on the other's products.
-//   warps 0..3, 4..7  softmax of half 0, 1: also load Q, write the output
+//   warps 0..3, 4..7  softmax of half 0, 1, and its output
 //   warp 8            TMA: pages' K and V rows into a ring of tiles
 //   warps 9, 10       issue the MMAs of half 0, 1 in turn: one waits for its
 //                     operands while the other issues, and the turn keeps the
 //                     halves out of step (without it both softmaxes ran at once
 //                     and then both products: 4500 clocks a unit)
+//   warp 11           TMA: the next item's queries, as soon as the last S of the
+//                     item before is there
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
 // last time (the sums carry the same factor, so the result is the same); MMAs
 // of one thread run in order, so when S of a tile is there, all products
@@ -46,7 +48,8 @@ struct Layout {
     static constexpr uint32_t kGroup = kParts * 1024u;   // 8 rows: [part][8][128 bytes], as the pages' boxes arrive
     static constexpr uint32_t kBytes = 16u * kGroup;     // a Q half, a K tile or a V tile: 128 rows
     static constexpr uint32_t kStages = 4u * 128u / D;        // K and V tiles in the ring: 128 KB
-    static constexpr uint32_t kRing = 2u * kBytes;            // after the two Q halves
+    static constexpr uint32_t kQPart = 128u * 128u;      // Q: [part][128 rows][128 bytes]
+    static constexpr uint32_t kRing = 2u * kBytes;       // after the two Q halves
     static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
 };
 
@@ -126,6 +129,40 @@ __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
+// The 4 x 4 blocks of 16 bytes of four neighbouring lanes, transposed: v[k] of lane j becomes v[j] of lane k.
+__device__ __forceinline__ void transpose4(uint4 (&v)[4], uint32_t lane) {
+#pragma unroll
+    for (uint32_t d = 1; d <= 2u; d <<= 1) {
+        const bool up = lane & d;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            if (k & d) continue;
+            uint4& a = v[k];
+            uint4& b = v[k | d];
+            const uint4 give = up ? a : b;
+            uint4 get;
+            get.x = __shfl_xor_sync(0xffffffffu, give.x, d);
+            get.y = __shfl_xor_sync(0xffffffffu, give.y, d);
+            get.z = __shfl_xor_sync(0xffffffffu, give.z, d);
+            get.w = __shfl_xor_sync(0xffffffffu, give.w, d);
+            if (up)
+                a = get;
+            else
+                b = get;
+        }
+    }
+}
+
+// Box of the queries' tensor (64 dims, 64-dim parts, heads, rows): packed rows of one part.
+__device__ __forceinline__ void tma_queries(void* dst, const CUtensorMap* map, int part, int head, int row,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(part), "r"(head), "r"(row), "r"(smem_addr(bar))
+        : "memory");
+}
+
 // ---- packed pairs of fp32 ------------------------------------------------------
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -190,13 +227,13 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                            PageMap heads, Args a, uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
+                            const __grid_constant__ CUtensorMap qmap, PageMap heads, Args a, uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
                             unsigned int* err) {
     using L = Layout<D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
-    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], s_full[2], p_full[2], o_full[2], turn[2], done;
+    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], turn[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
@@ -204,7 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (uint32_t s = 0; s < L::kStages; ++s) mbar_init(&kv_full[s], 1), mbar_init(&kv_empty[s], 2);
         for (uint32_t s = 0; s < 2; ++s) {
-            mbar_init(&q_full[s], 4);
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], 1);
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 4);
             mbar_init(&o_full[s], 1);
@@ -358,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kQk = instr_desc<BF16>(128, false), kPv = instr_desc<BF16>(D, true);
         const uint32_t s = warp - 9u, leader = lane == 0;
         const uint32_t ring = smem_addr(smem + L::kRing), ts = tmem + s * 128u, to = tmem + 256u + s * 128u;
-        const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kBytes, 16u, L::kGroup);
+        const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kBytes, 16u, 1024u);
         uint32_t stage = 0, phase = 0, n_item = 0, n_p = 0, n_turn = s ^ 1u;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = role_wait(bar, parity, &abort_flag, err); };
@@ -377,8 +415,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t kb = operand_desc(ring + k_stage * L::kBytes, 16u, L::kGroup);
 #pragma unroll
             for (uint32_t kk = 0; kk < D / 16u; ++kk) {
-                const uint32_t o = ((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4;  // addresses count 16 bytes
-                mma_smem(ts, qa + o, kb + o, kQk, kk != 0u, leader);
+                // addresses count 16 bytes
+                mma_smem(ts, qa + (((kk >> 2) * L::kQPart + (kk & 3u) * 32u) >> 4),
+                         kb + (((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4), kQk, kk != 0u, leader);
             }
             mma_commit(&s_full[s], leader);
         };
@@ -390,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!my_turn()) break;
             if (live) qk(stage);
             pass_turn();
+            if (live && i1 - i0 == 1u) mma_commit(&q_empty[s], leader);
             mma_commit(&kv_empty[stage], leader);
             advance();
             for (uint32_t i = i0; i < i1; ++i) {
@@ -435,6 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         mma_commit(&o_full[s], leader);
                 }
                 pass_turn();
+                if (live && i + 2u == i1) mma_commit(&q_empty[s], leader);  // the last S has been issued
                 mma_commit(&kv_empty[v_stage], leader);
                 if (more) mma_commit(&kv_empty[k_stage], leader);
             }
@@ -443,6 +484,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(&done, leader);
         __syncwarp();
         mbar_wait(&done, 0, err);  // nothing of this CTA runs on the tensor core any more
+      } else {
+        // ---------------- TMA: queries ----------------
+        uint32_t n[2] = {0, 0};
+        bool ok = true;
+        do {
+#pragma unroll
+            for (uint32_t s = 0; s < 2u; ++s) {
+                if (s * half_rows >= w.rows) continue;
+                if (n[s] != 0u) ok = ok && role_wait(&q_empty[s], (n[s] - 1u) & 1u, &abort_flag, err);
+                if (!ok) continue;
+                ++n[s];
+                if (lane == 0) {  // rows past the request's are other requests' or zeros: computed, not stored
+                    mbar_arrive_expect_tx(&q_full[s], L::kParts * half_rows * a.gq * 128u);
+#pragma unroll
+                    for (uint32_t c = 0; c < L::kParts; ++c)
+                        tma_queries(smem + s * L::kBytes + c * L::kQPart, &qmap, (int)c, (int)(w.kvh * a.gq),
+                                    (int)(w.q.row0 + w.first + s * half_rows), &q_full[s]);
+                }
+                __syncwarp();
+            }
+        } while (ok && w.next(a, off, per_item));
+        if (!ok) abort_flag = 1;
+#pragma unroll
+        for (uint32_t s = 0; s < 2u; ++s)  // no copy may still be landing at the end
+            if (n[s] != 0u) mbar_wait(&q_full[s], (n[s] - 1u) & 1u, err);
       }
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -452,37 +518,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t ts = tmem + lanes + s * 128u, to = tmem + lanes + 256u + s * 128u;
         uint32_t n_s = 0, n_o = 0;
-        const uint32_t t_row = t / a.gq, t_head = t - t_row * a.gq;
-        // Row t of Q, when the half has rows in the item; its place is free once S of the item before is there.
-        auto load_q = [&](const Walk& x) {
-            if (s * half_rows >= x.rows) return;
-            const bool live = t_row < min(half_rows, x.rows - s * half_rows);
-            const uint4* src = reinterpret_cast<const uint4*>(
-                a.q + (uint64_t)(x.q.row0 + x.first + s * half_rows + (live ? t_row : 0u)) * a.q_stride +
-                (x.kvh * a.gq + t_head) * D);
-            uint8_t* dst = smem + s * L::kBytes + (t >> 3) * L::kGroup + (t & 7u) * 128u;
-#pragma unroll
-            for (uint32_t c = 0; c < D / 8u; ++c) {
-                const uint4 v = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * 1024u + (((c & 7u) ^ (t & 7u)) << 4)) = v;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[s]);
-        };
-        load_q(w);
+        const uint32_t t_row = t / a.gq;
         bool ok = true;
         for (bool more = true; more;) {
             const uint32_t i0 = w.begin(), i1 = w.end();
-            Walk nw = w;
             if (s * half_rows >= w.rows) {  // this half has no rows (uniform over its warps)
-                more = nw.next(a, off, per_item);
-                if (more) load_q(nw);
-                w = nw;
+                more = w.next(a, off, per_item);
                 continue;
             }
             const uint32_t sub_rows = min(half_rows, w.rows - s * half_rows);
             const uint32_t p_lo = w.lo + s * half_rows, p_hi = p_lo + sub_rows - 1u;
+            const bool live = t_row < sub_rows;
             const uint32_t pos = p_lo + min(t_row, sub_rows - 1u);
             float m = -INFINITY, l = 0.f;
             for (uint32_t i = i0; i < i1; ++i) {
@@ -500,31 +546,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // 64 columns at a time in a loop that stays one: tensor memory gives 128 columns in 90 clocks, so S is
                 // read twice rather than kept in 128 registers, and the code of all roles stays small enough for the
                 // instruction caches, which straight-line code for 128 columns was not.
-                auto columns = [&](uint32_t c0, float (&x)[64]) {
-                    tmem_ld64(ts + c0, x);
-                    if (past || before) {
-                        const int e = last - (int)c0, f = first - (int)c0, g = sinks - (int)c0;
-#pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c > e || (c < f && c >= g)) x[c] = -INFINITY;
-                    }
-                };
                 float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
                 for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
                     float x[64];
-                    columns(c0, x);
+                    tmem_ld64(ts + c0, x);
+                    if (past || before) {  // -inf where the row does not see, also for the second reading
+                        const int e = last - (int)c0, f = first - (int)c0, g = sinks - (int)c0;
+                        if (before) {
+#pragma unroll
+                            for (int c = 0; c < 64; ++c)
+                                if (c < f && c >= g) x[c] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (c > e) x[c] = -INFINITY;
+                        tmem_st64(ts + c0, x);
+                    }
 #pragma unroll
                     for (uint32_t c = 0; c < 64u; c += 4u)
 #pragma unroll
                         for (uint32_t k = 0; k < 2u; ++k) mx[k] = max_nan(mx[k], x[c + 2u * k], x[c + 2u * k + 1u]);
                 }
+                if (past || before) tmem_wait_st();
                 // An infinite score has no softmax: NaN for the row, as for a NaN score.
                 float mn = max_nan(mx[0], mx[1]) * a.scale_log2;
                 if (mn == INFINITY) mn = NAN;
                 if (i == i0) {
                     m = mn;  // O is written afresh
-                } else if (__any_sync(0xffffffffu, !(mn <= m + kGrow))) {
+                } else if (__any_sync(0xffffffffu, live && !(mn <= m + kGrow))) {
                     const float to_m = max_nan(m, mn);
                     const float f = ex2(m - (to_m == -INFINITY ? 0.f : to_m));
                     l *= f;
@@ -545,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
                     float x[64];
-                    columns(c0, x);
+                    tmem_ld64(ts + c0, x);
                     uint32_t pk[32];
 #pragma unroll
                     for (uint32_t c = 0; c < 64u; c += 2u) {
@@ -570,35 +620,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[s]);
             }
-            // The next item's Q goes in while the last product runs; its S may follow at once, its O only after
-            // this thread has handed over weights, and by then it has read O.
-            if (ok) {
-                more = nw.next(a, off, per_item);
-                if (more) load_q(nw);
-                ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
-            }
+            if (ok) ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
             if (!ok) break;
             ++n_o;
             tmem_fence_after();
-            const bool whole = i0 == 0 && i1 == w.s.n, live = t_row < sub_rows;
+            const bool whole = i0 == 0 && i1 == w.s.n;
             const uint32_t slot = i0 != 0 ? 0u : 1u;  // began before this stretch, or goes on after it
             float* part = parts + (uint64_t)(blockIdx.x * 2u + slot) * (kTileRows * (D + 2u));
             const uint32_t ri = s * half_rows * a.gq + t;
-            uint16_t* out = a.out + (uint64_t)(w.q.row0 + w.first + s * half_rows + t_row) * a.out_stride +
-                            (w.kvh * a.gq + t_head) * D;
+            uint16_t* out_of[4];  // rows of this thread and its three neighbours
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t tk = (t & ~3u) + k, row = tk / a.gq;
+                out_of[k] = row < sub_rows
+                                ? a.out + (uint64_t)(w.q.row0 + w.first + s * half_rows + row) * a.out_stride +
+                                      (w.kvh * a.gq + tk - row * a.gq) * D
+                                : nullptr;
+            }
             const float inv = 1.f / l;
 #pragma unroll 1
             for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
                 float o[32];
                 tmem_ld32(to + c, o);
-                if (live && whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(out + c);
+                if (whole) {
+                    // 16 bytes of each of four neighbours' rows instead of 64 of its own: a store then touches 8 rows
+                    // of 64 bytes rather than 32 of 16
+                    uint4 v[4];
 #pragma unroll
                     for (uint32_t k = 0; k < 4u; ++k)
-                        dst[k] = make_uint4(pack16<BF16>(o[8 * k] * inv, o[8 * k + 1] * inv),
-                                            pack16<BF16>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                                            pack16<BF16>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
-                                            pack16<BF16>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                        v[k] = make_uint4(pack16<BF16>(o[8 * k] * inv, o[8 * k + 1] * inv),
+                                          pack16<BF16>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                          pack16<BF16>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
+                                          pack16<BF16>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                    transpose4(v, lane);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k)
+                        if (out_of[k] != nullptr) *reinterpret_cast<uint4*>(out_of[k] + c + (lane & 3u) * 8u) = v[k];
                 } else if (live) {
                     float4* dst = reinterpret_cast<float4*>(part + (uint64_t)ri * D + c);
 #pragma unroll
@@ -614,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     recs[blockIdx.x] = {1u, (U0 + n_units - w.left - w.v + kItemCost + w.s.n - 1u) / per, w.q.row0 + w.first, w.rows * a.gq, w.kvh,
                                         {0, 0, 0}};
             }
-            w = nw;
+            more = w.next(a, off, per_item);
         }
         if (!ok) abort_flag = 1;
       }
@@ -635,12 +692,24 @@ int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, fl
     PageMap heads;
     const int st = encode_pages(&kmap, &vmap, &heads, kv, box);
     if (st != ARC_OK) return st;
+    CUtensorMap qmap;
+    {
+        const uint32_t q_heads = a.kv_heads * a.gq;
+        const cuuint64_t dims[4] = {64, L::kParts, q_heads, a.max_rows};
+        const cuuint64_t strides[3] = {128, 2ull * D, 2ull * a.q_stride};
+        const cuuint32_t shape[4] = {64, 1, a.gq, 128u / a.gq}, one[4] = {1, 1, 1, 1};
+        const CUresult rc = encode_tiled_fn()(
+            &qmap, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<uint16_t*>(a.q), dims, strides, shape, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (rc != CUDA_SUCCESS) return set_error(ARC_E_CUDA, "attention paged: tensor map of the queries");
+    }
     const uint32_t smem = 1024u + L::kOff + 4u * (a.n_requests + 1u);
     cudaError_t e = cudaFuncSetAttribute(attn_paged_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
     if (e == cudaSuccess)
         e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap,
-                          heads, a, box, 1u, recs, parts, dev_error_word());
+                          qmap, heads, a, box, 1u, recs, parts, dev_error_word());
     return e == cudaSuccess ? ARC_OK : set_cuda_error(e, "attention paged tiles launch");
 }
 
