@@ -5,7 +5,6 @@
 // (arcllm_cuda_argmax is the choice without them).
 #include <algorithm>
 
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "arcllm_cuda_internal.h"
@@ -17,8 +16,9 @@ namespace arc {
 namespace {
 
 constexpr uint32_t kLogitsThreads = 512;
-constexpr uint32_t kLogitsCluster = 8;      // CTAs per row
-constexpr uint32_t kLogitsWords = 20480;    // per-token words of a chunk in shared memory (80 KB: two CTAs per SM)
+constexpr uint32_t kChunk = 131072;  // most tokens a CTA takes at a time: two words of shared memory for 32
+constexpr uint32_t kNamed = 4096;    // most named tokens whose words are held at a time
+constexpr uint32_t kList = 4096;     // history entries of the chunk that are kept in shared memory
 constexpr uint32_t kPromptSeen = 0x80000000u;
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -52,36 +52,85 @@ __device__ __forceinline__ float constrained(float x, uint32_t word, const RowPa
     return x;
 }
 
-// A cluster of 8 CTAs per row, each over a contiguous eighth of the
-// vocabulary.  Per chunk of its slice a CTA counts the row's history into
-// shared memory (one word per token: generated count, top bit: in the prompt;
-// with biases a second word: 1 + the index of the token's last entry), then
-// streams the logits through once: read, constrain, round, write, and keep the
-// best finite value with the lowest index.  The eight bests meet in CTA 0
-// through distributed shared memory, so no workspace, no atomics on global
-// memory and no order of arrival is involved.  Many rows: HBM traffic of the
-// logits in and out; one row: 8 CTAs, latency.
+struct Best {
+    float v = -INFINITY;
+    uint32_t at = 0xffffffffu;
+};
+
+// One 64-bit word into another CTA's shared memory, counted by a barrier there.
+__device__ __forceinline__ void st_async_u64(uint32_t addr, unsigned long long v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(addr), "l"(v), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {  // the same place in CTA `rank`
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+    return r;
+}
+
+// A cluster of 1 to 16 CTAs per row, each over a contiguous part of the
+// vocabulary.  The tokens that the row's history or biases name are few: they are
+// marked by one bit each, and the number of bits before a token's own is the
+// place of its words (generated count, top bit: in the prompt; with biases 1 +
+// the index of its last entry), so shared memory holds words for the named tokens
+// only and a CTA's part can be long.  The history is read once, its entries of
+// the part kept in a list.  Then one stream over the logits reads, constrains,
+// masks and writes them and keeps the best finite value with the lowest index.
+// The CTAs' bests go to CTA 0's shared memory by asynchronous stores (a cluster
+// barrier would first drain every store: 4000 clocks), so no workspace, no
+// atomics on global memory and no order of arrival is involved.
+// Many rows: HBM traffic of the logits in and out; finishing the named tokens
+// after the stream, with loads of their own, cost a third of its time again, and
+// bulk copies into shared memory ahead of it were slower than the loads in
+// registers.  One row: latency.
 template <typename T, int V>
 __global__ void __launch_bounds__(kLogitsThreads, 2)
-    logits_process_kernel(LogitsProcess p, uint32_t slice, uint32_t chunk) {
+    logits_process_kernel(LogitsProcess p, uint32_t slice, uint32_t chunk, unsigned int* err) {
+    extern __shared__ uint32_t smem[];  // named bits, bits before each word's, list; counts, last bias entries
+    __shared__ unsigned long long s_best[kLogitsThreads / 32], s_keys[16];
+    __shared__ uint64_t keys_in;
+    __shared__ uint32_t s_sum[kLogitsThreads / 32], s_listed;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, row = blockIdx.y;
+    if (tid == 0) {
+        mbar_init(&keys_in, 1);
+        mbar_arrive_expect_tx(&keys_in, 8u * (gridDim.x - 1u));
+        fence_mbar_init();
+    }
+    if (gridDim.x > 1u) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_trigger();
     pdl_wait();  // logits come from the preceding kernels
-    namespace cg = cooperative_groups;
-    cg::cluster_group cl = cg::this_cluster();
-    extern __shared__ uint32_t words[];
-    __shared__ unsigned long long s_best[kLogitsThreads / 32];
-    __shared__ unsigned long long s_key;
-    const uint32_t tid = threadIdx.x, row = blockIdx.y;
     const uint32_t v_begin = min(blockIdx.x * slice, p.vocab), v_end = min(v_begin + slice, p.vocab);
     const T* in = static_cast<const T*>(p.logits) + (uint64_t)row * p.stride;
     T* out = static_cast<T*>(p.out) + (uint64_t)row * p.out_stride;
+    constexpr uint32_t U = 4;  // vectors in flight per thread
+    T x[U][V];
+    auto load = [&](uint32_t i0, uint32_t i1) {  // of the part's tokens [i0, i1)
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j) {
+            const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
+            if (i + V <= i1) {
+                if constexpr (V > 1)
+                    *reinterpret_cast<uint4*>(x[j]) = __ldcs(reinterpret_cast<const uint4*>(in + i));
+                else
+                    x[j][0] = in[i];
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < V; ++k)
+                    if (i + k < i1) x[j][k] = in[i + k];
+            }
+        }
+    };
+    load(v_begin, v_end);  // on their way while the tokens are counted
     RowParams rp;
     rp.has_rep = p.repetition != nullptr, rp.has_freq = p.frequency != nullptr, rp.has_pres = p.presence != nullptr;
+    const bool penalties = p.history && (rp.has_rep || rp.has_freq || rp.has_pres);
+    const int32_t* hist = p.history + (uint64_t)row * p.history_stride;
+    const uint32_t* mask = p.mask ? p.mask + (uint64_t)row * p.mask_stride : nullptr;
     rp.rep = rp.has_rep ? p.repetition[row] : 1.f;
     rp.freq = rp.has_freq ? p.frequency[row] : 0.f;
     rp.pres = rp.has_pres ? p.presence[row] : 0.f;
     uint32_t n_hist = 0, n_prompt = 0, b0 = 0, b1 = 0;
-    if (p.history && (rp.has_rep || rp.has_freq || rp.has_pres)) {
+    if (penalties) {
         n_hist = (uint32_t)min(max(p.total_len[row], 0), (int32_t)p.history_stride);
         n_prompt = p.prompt_len ? (uint32_t)max(p.prompt_len[row], 0) : 0u;
     }
@@ -89,119 +138,219 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
         b0 = (uint32_t)max(p.bias_start[row], 0);
         b1 = (uint32_t)max(p.bias_start[row + 1], (int32_t)b0);
     }
-    const int32_t* hist = p.history + (uint64_t)row * p.history_stride;
-    const uint32_t* mask = p.mask ? p.mask + (uint64_t)row * p.mask_stride : nullptr;
-    uint32_t* count = words;
-    uint32_t* last = words + chunk;  // only with biases
-    float best = -INFINITY;
-    uint32_t best_at = 0xffffffffu;
+    const uint32_t n_words = (chunk + 31u) / 32u;
+    uint32_t* named = smem;
+    uint32_t* before = named + n_words;
+    uint32_t* list = before + n_words + 1u;  // token - chunk's first, top bit: of the prompt
+    uint32_t* count = list + kList;
+    uint32_t* last = count + kNamed;  // only with biases
+    const bool any = n_hist != 0u || b1 != b0;
+    Best best;
     for (uint32_t c0 = v_begin; c0 < v_end; c0 += chunk) {
         const uint32_t n = min(chunk, v_end - c0);
-        const bool counted = n_hist != 0u, biased = b1 != b0;
-        if (counted || biased) {
-            for (uint32_t i = tid; i < n; i += kLogitsThreads) {
-                if (counted) count[i] = 0u;
-                if (biased) last[i] = 0u;
-            }
+        uint32_t n_named = 0, n_listed = 0;
+        if (any) {
+#pragma unroll 1
+            for (uint32_t i = tid; i < n_words; i += kLogitsThreads) named[i] = 0u;
+            if (tid == 0) s_listed = 0u;
             __syncthreads();
-            for (uint32_t i = tid; i < n_hist; i += kLogitsThreads) {
-                const uint32_t id = (uint32_t)hist[i] - c0;  // outside the chunk, or no token: a large number
-                if (id < n) {
-                    if (i < n_prompt)
-                        atomicOr(&count[id], kPromptSeen);
-                    else
-                        atomicAdd(&count[id], 1u);
+            auto name = [&](uint32_t i) {
+                const uint32_t bit = 1u << (i & 31u);
+                if (!(*(volatile uint32_t*)&named[i >> 5] & bit)) atomicOr(&named[i >> 5], bit);
+            };
+            constexpr uint32_t E = 4;  // entries on their way together
+#pragma unroll 1
+            for (uint32_t e0 = 0; e0 < n_hist; e0 += kLogitsThreads * E) {
+                uint32_t id[E];
+#pragma unroll
+                for (uint32_t k = 0; k < E; ++k) {
+                    const uint32_t e = e0 + k * kLogitsThreads + tid;
+                    id[k] = e < n_hist ? (uint32_t)__ldg(hist + e) - c0 : n;  // >= n: none of the chunk
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < E; ++k) {
+                    const uint32_t e = e0 + k * kLogitsThreads + tid, here = __ballot_sync(0xffffffffu, id[k] < n);
+                    uint32_t at = 0;
+                    if (here && lane == 0) at = atomicAdd(&s_listed, (uint32_t)__popc(here));
+                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(here & ((1u << lane) - 1u));
+                    if (id[k] >= n) continue;
+                    name(id[k]);
+                    if (at < kList) list[at] = id[k] | (e < n_prompt ? kPromptSeen : 0u);
                 }
             }
-            for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads) {
-                const uint32_t id = (uint32_t)p.bias_ids[e] - c0;
-                if (id < n) atomicMax(&last[id], e - b0 + 1u);
-            }
+#pragma unroll 1
+            for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads)
+                if (const uint32_t i = (uint32_t)p.bias_ids[e] - c0; i < n) name(i);
             __syncthreads();
-        }
-        constexpr uint32_t U = 4;  // vectors in flight per thread
-        for (uint32_t i0 = 0; i0 < n; i0 += kLogitsThreads * V * U) {
-            T x[U][V];
+            n_listed = s_listed;
+            const uint32_t per = (n_words + kLogitsThreads - 1u) / kLogitsThreads;
+            const uint32_t w0 = min(tid * per, n_words), w1 = min(w0 + per, n_words);
+            uint32_t mine = 0;
+#pragma unroll 1
+            for (uint32_t i = w0; i < w1; ++i) mine += __popc(named[i]);
+            uint32_t sum = mine;
 #pragma unroll
-            for (uint32_t j = 0; j < U; ++j) {
-                const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
-                if (i + V <= n) {
-                    if constexpr (V > 1)
-                        *reinterpret_cast<uint4*>(x[j]) = __ldcs(reinterpret_cast<const uint4*>(in + c0 + i));
-                    else
-                        x[j][0] = in[c0 + i];
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < V; ++k)
-                        if (i + k < n) x[j][k] = in[c0 + i + k];
-                }
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= (uint32_t)o) sum += y;
             }
+            if (lane == 31u) s_sum[warp] = sum;
+            __syncthreads();
+            sum -= mine;
 #pragma unroll
-            for (uint32_t j = 0; j < U; ++j) {
-                const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
-                if (i >= n) continue;
-                // V consecutive tokens start on a multiple of V, so their mask bits lie in one word
-                const uint32_t allowed = mask ? mask[(c0 + i) >> 5] >> ((c0 + i) & 31u) : 0xffffffffu;
-#pragma unroll
-                for (uint32_t k = 0; k < V; ++k) {
-                    if (i + k >= n) continue;
-                    float v = constrained(to_f32(x[j][k]), counted ? count[i + k] : 0u, rp);
-                    if (biased && last[i + k]) v = __fadd_rn(v, p.bias_values[b0 + last[i + k] - 1u]);
-                    if (!((allowed >> k) & 1u)) v = -INFINITY;
-                    from_f32(v, x[j][k]);
-                    v = to_f32(x[j][k]);
-                    if (isfinite(v) && (v > best || best_at == 0xffffffffu)) best = v, best_at = c0 + i + k;
-                }
-                if (i + V <= n) {
-                    if constexpr (V > 1)
-                        __stcs(reinterpret_cast<uint4*>(out + c0 + i), *reinterpret_cast<const uint4*>(x[j]));
-                    else
-                        out[c0 + i] = x[j][0];
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < V; ++k)
-                        if (i + k < n) out[c0 + i + k] = x[j][k];
-                }
+            for (uint32_t w = 0; w < kLogitsThreads / 32; ++w) {
+                if (w < warp) sum += s_sum[w];
+                n_named += s_sum[w];
+            }
+#pragma unroll 1
+            for (uint32_t i = w0; i < w1; ++i) {
+                before[i] = sum;
+                sum += __popc(named[i]);
             }
         }
-        if (c0 + chunk < v_end) __syncthreads();  // the words are filled anew
-    }
-    if (!p.best) return;
-    unsigned long long key =
-        best_at == 0xffffffffu ? 0ull : ((unsigned long long)ordered(best) << 32) | (unsigned long long)(~best_at);
+        if (any && tid == 0) before[n_words] = n_named;
+        // As many words of bits at a time as name kNamed tokens at most (nearly always all of them).
+        for (uint32_t w0 = 0; w0 * 32u < n;) {
+            uint32_t w1 = n_words, first = 0;
+            if (n_named) {
+                __syncthreads();  // `before` is complete; the words of the round before are done with
+                first = before[w0];
+                if (n_named - first > kNamed) {
+                    uint32_t lo = w0;  // before[lo] <= first + kNamed < before[w1]
+                    while (w1 - lo > 1u) {
+                        const uint32_t mid = (lo + w1) / 2u;
+                        if (before[mid] <= first + kNamed)
+                            lo = mid;
+                        else
+                            w1 = mid;
+                    }
+                    w1 = lo;
+                }
+                const uint32_t held = before[w1] - first;
+                for (uint32_t i = tid; i < held; i += kLogitsThreads) {
+                    count[i] = 0u;
+                    if (p.bias_start) last[i] = 0u;
+                }
+                __syncthreads();
+            }
+            auto place = [&](uint32_t i) {  // of a named token of these words
+                const uint32_t w = i >> 5;
+                return before[w] + __popc(named[w] & ((1u << (i & 31u)) - 1u)) - first;
+            };
+            const uint32_t s0 = w0 * 32u, s1 = min(w1 * 32u, n);
+            if (n_named) {
+                const bool listed = n_listed <= kList;  // otherwise the history is read again
+                const uint32_t entries = listed ? n_listed : n_hist;
+#pragma unroll 1
+                for (uint32_t e = tid; e < entries; e += kLogitsThreads) {
+                    const uint32_t entry = listed ? list[e] : (uint32_t)__ldg(hist + e) - c0;
+                    const bool prompt = listed ? (entry & kPromptSeen) != 0u : e < n_prompt;
+                    const uint32_t i = listed ? entry & ~kPromptSeen : entry;
+                    if (i < s0 || i >= s1) continue;
+                    uint32_t* word = &count[place(i)];
+                    if (!prompt)
+                        atomicAdd(word, 1u);
+                    else if (!(*(volatile uint32_t*)word & kPromptSeen))
+                        atomicOr(word, kPromptSeen);
+                }
+#pragma unroll 1
+                for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads)
+                    if (const uint32_t i = (uint32_t)p.bias_ids[e] - c0; i >= s0 && i < s1)
+                        atomicMax(&last[place(i)], e - b0 + 1u);
+                __syncthreads();
+            }
+#pragma unroll 1
+            for (uint32_t i0 = s0; i0 < s1; i0 += kLogitsThreads * V * U) {
+                if (c0 + i0 != v_begin) load(c0 + i0, c0 + s1);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-        key = other > key ? other : key;
-    }
-    if ((tid & 31u) == 0) s_best[tid >> 5] = key;
-    __syncthreads();
-    if (tid == 0) {
+                for (uint32_t j = 0; j < U; ++j) {
+                    const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
+                    if (i >= s1) continue;
+                    // V consecutive tokens start on a multiple of V, so their bits lie in one word
+                    const uint32_t allowed = mask ? __ldg(mask + ((c0 + i) >> 5)) >> ((c0 + i) & 31u) : 0xffffffffu;
+                    const uint32_t here = n_named ? (named[i >> 5] >> (i & 31u)) & ((1u << V) - 1u) : 0u;
+                    if (here) {
+                        uint32_t r = place(i);
 #pragma unroll
-        for (uint32_t w = 1; w < kLogitsThreads / 32; ++w) key = s_best[w] > key ? s_best[w] : key;
-        s_key = key;
+                        for (uint32_t k = 0; k < V; ++k) {
+                            if (!((here >> k) & 1u)) continue;
+                            float v = constrained(to_f32(x[j][k]), count[r], rp);
+                            if (p.bias_start && last[r]) v = __fadd_rn(v, p.bias_values[b0 + last[r] - 1u]);
+                            from_f32(v, x[j][k]);
+                            ++r;
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < V; ++k) {
+                        if (i + k >= s1) continue;
+                        if (!((allowed >> k) & 1u))
+                            from_f32(-INFINITY, x[j][k]);
+                        else if (const float v = to_f32(x[j][k]); v > best.v && v < INFINITY)
+                            best.v = v, best.at = c0 + i + k;  // tokens ascend, so the first of equals stays
+                    }
+                    if (i + V <= s1) {
+                        if constexpr (V > 1)
+                            __stcs(reinterpret_cast<uint4*>(out + c0 + i), *reinterpret_cast<const uint4*>(x[j]));
+                        else
+                            out[c0 + i] = x[j][0];
+                    } else {
+#pragma unroll
+                        for (uint32_t k = 0; k < V; ++k)
+                            if (i + k < s1) out[c0 + i + k] = x[j][k];
+                    }
+                }
+            }
+            w0 = w1;
+        }
+        if (c0 + chunk < v_end) __syncthreads();  // bits and list are set anew
     }
-    cl.sync();
-    if (cl.block_rank() == 0 && tid == 0) {
-        for (uint32_t c = 1; c < kLogitsCluster; ++c) {
-            const unsigned long long other = *cl.map_shared_rank(&s_key, c);
+    if (p.best) {
+        unsigned long long key = best.at == 0xffffffffu
+                                     ? 0ull
+                                     : ((unsigned long long)ordered(best.v) << 32) | (unsigned long long)(~best.at);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
             key = other > key ? other : key;
         }
-        p.best[row] = key ? (int32_t)~(uint32_t)(key & 0xffffffffull) : -1;
+        if (lane == 0) s_best[warp] = key;
+        __syncthreads();
+        if (tid == 0)
+#pragma unroll
+            for (uint32_t w = 1; w < kLogitsThreads / 32; ++w) key = s_best[w] > key ? s_best[w] : key;
+        if (gridDim.x > 1u) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // CTA 0 is ready
+        if (tid == 0 && blockIdx.x != 0)
+            st_async_u64(shared_of(&s_keys[blockIdx.x], 0), key, shared_of(&keys_in, 0));
+        if (tid == 0 && blockIdx.x == 0) {
+            if (gridDim.x > 1u && mbar_wait(&keys_in, 0, err))
+                for (uint32_t c = 1; c < gridDim.x; ++c) key = s_keys[c] > key ? s_keys[c] : key;
+            p.best[row] = key ? (int32_t)~(uint32_t)(key & 0xffffffffull) : -1;
+        }
+    } else if (gridDim.x > 1u) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    cl.sync();  // no CTA leaves while CTA 0 still reads its key
 }
 
 template <typename T, int V>
 cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, cudaStream_t stream) {
+    // CTAs per row: as many as give the least waves x (tokens of a CTA + what a CTA costs beside them)
+    constexpr uint64_t kSlots = 2u * 148u, kCtaCost = 7500u;
+    uint32_t ctas = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t c = 1; c <= 16u; c *= 2u) {
+        const uint64_t t = ((uint64_t)p.n_rows * c + kSlots - 1u) / kSlots * (p.vocab / c + kCtaCost);
+        if (t < least) least = t, ctas = c;
+    }
+    const uint32_t slice = ((p.vocab + ctas - 1u) / ctas + 31u) / 32u * 32u;
+    const uint32_t chunk = std::min(slice, kChunk);
     const bool counts = p.history && (p.repetition || p.frequency || p.presence);
-    const uint32_t slice = ((p.vocab + kLogitsCluster - 1u) / kLogitsCluster + 31u) / 32u * 32u;  // whole mask words
-    const uint32_t most = p.bias_start ? kLogitsWords / 2u : kLogitsWords;
-    const uint32_t parts = (slice + most - 1u) / most;
-    const uint32_t chunk = ((slice + parts - 1u) / parts + 31u) / 32u * 32u;
-    const uint32_t smem = p.bias_start ? 8u * chunk : counts ? 4u * chunk : 0u;
+    const uint32_t smem = counts || p.bias_start
+                              ? (chunk + 31u) / 32u * 8u + 4u + 4u * kList + 4u * kNamed * (p.bias_start ? 2u : 1u)
+                              : 0u;
     cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         4 * kLogitsWords);
+                                         kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(logits_process_kernel<T, V>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     LogitsProcess q = p;
     q.n_rows = rows;
@@ -218,13 +367,13 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
     q.mask = shift(p.mask, (uint64_t)row0 * p.mask_stride);
     q.best = shift(p.best, row0);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kLogitsCluster, rows);
+    cfg.gridDim = dim3(ctas, rows);
     cfg.blockDim = dim3(kLogitsThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kLogitsCluster;
+    attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -234,7 +383,7 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    e = cudaLaunchKernelEx(&cfg, logits_process_kernel<T, V>, q, slice, chunk);
+    e = cudaLaunchKernelEx(&cfg, logits_process_kernel<T, V>, q, slice, chunk, dev_error_word());
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -263,8 +412,8 @@ int logits_process(int type, const LogitsProcess& p, cudaStream_t stream) {
     if (p.vocab == 0 || p.vocab > 0x7fffffffu - 512u || p.n_rows > 0x7fffffffu || p.stride < p.vocab ||
         p.out_stride < p.vocab)
         return set_error(ARC_E_INVALID_ARGUMENT, "logits: bad shape");
-    if (p.history && (!p.total_len || p.history_stride > 0x3fffffffu))
-        return set_error(ARC_E_INVALID_ARGUMENT, "logits: a history needs total_len and a stride below 2^30");
+    if (p.history && (!p.total_len || p.history_stride > 0x1fffffffu))
+        return set_error(ARC_E_INVALID_ARGUMENT, "logits: a history needs total_len and a stride below 2^29");
     if ((p.repetition || p.frequency || p.presence) && !p.history)
         return set_error(ARC_E_INVALID_ARGUMENT, "logits: penalties need a history");
     if (p.bias_start && (!p.bias_ids || !p.bias_values))

@@ -204,106 +204,111 @@ __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
 // may be rotated in place.  Units of a head: rotated ones first.
 // Angles pos * freq are formed and reduced to a fraction of a turn in 64 bits
 // (at 16384 an fp32 product is already 1e-3 off), then sin and cos in fp32.
+// The row is read before its slot and position are known, so that the loads are
+// on their way together (rows without a request are read for nothing).
 // Bounded by HBM traffic for many rows and by latency for few.
+constexpr uint32_t kRopeThreads = 512;
 template <typename TA, typename TC, int V>
-__global__ void __launch_bounds__(256) rope_kv_paged_kernel(RopePaged p, arcllm_cuda_paged_kv kv, unsigned int* err) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kv_paged_kernel(RopePaged p, arcllm_cuda_paged_kv kv,
+                                                                     unsigned int* err) {
     pdl_trigger();
     pdl_wait();  // q, k, v come from the preceding kernels
     extern __shared__ float2 rope_smem[];  // (cos, sin) * attn_scale of the row's rot_dim / 2 pairs
-    const uint32_t row = blockIdx.x;
+    const uint32_t row = blockIdx.x, d = kv.head_dim, half = p.rot_dim / 2u;
+    const uint32_t per_head = d / (2u * V), rot_units = half / V, rot_heads = p.q_heads + kv.kv_heads;
+    const uint32_t units = (rot_heads + kv.kv_heads) * per_head, step = gridDim.y * blockDim.x;
+    struct Unit {
+        uint32_t head, oa, ob, w;  // head of q, k, v in a row; places of the vectors in it; number in the head
+        float a[V], b[V];
+        const float* bias;
+    } x;
+    auto load = [&](uint32_t u) {
+        x.head = u / per_head;
+        x.w = u - x.head * per_head;
+        const bool halves = p.half_layout && x.w < rot_units && x.head < rot_heads;
+        x.oa = halves ? x.w * V : 2u * x.w * V;
+        x.ob = halves ? half + x.w * V : x.oa + V;
+        const TA* src;
+        if (x.head < p.q_heads) {
+            src = static_cast<const TA*>(p.q) + (uint64_t)row * p.q_stride + x.head * d;
+            x.bias = p.bq ? p.bq + x.head * d : nullptr;
+        } else if (x.head < rot_heads) {
+            src = static_cast<const TA*>(p.k) + (uint64_t)row * p.k_stride + (x.head - p.q_heads) * d;
+            x.bias = p.bk ? p.bk + (x.head - p.q_heads) * d : nullptr;
+        } else {
+            src = static_cast<const TA*>(p.v) + (uint64_t)row * p.v_stride + (x.head - rot_heads) * d;
+            x.bias = p.bv ? p.bv + (x.head - rot_heads) * d : nullptr;
+        }
+        load_vec<V>(src + x.oa, x.a);
+        load_vec<V>(src + x.ob, x.b);
+        if (x.bias) {
+            float ba[V], bb[V];
+            load_vec<V>(x.bias + x.oa, ba);
+            load_vec<V>(x.bias + x.ob, bb);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x.a[i] += ba[i], x.b[i] += bb[i];
+        }
+    };
+    uint32_t u = blockIdx.y * blockDim.x + threadIdx.x;
+    if (u < units) load(u);
     const int32_t slot = p.slots[row], pos = p.positions[row];
     if (slot < 0) return;  // a row without a request (uniform over the CTA)
     if ((uint32_t)slot >= kv.n_pages * kv.page_size || pos < 0) {
         if (threadIdx.x == 0 && blockIdx.y == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
         return;
     }
-    const uint32_t d = kv.head_dim, half = p.rot_dim / 2u;
-    const uint32_t per_head = d / (2u * V), rot_units = half / V;
-    const uint32_t units = (p.q_heads + 2u * kv.kv_heads) * per_head;
+    for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
+        const double turns = (double)pos * p.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
+        float s, c;
+        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+        rope_smem[i] = make_float2(c * p.attn_scale, s * p.attn_scale);
+    }
+    __syncthreads();
     const uint32_t page = (uint32_t)slot / kv.page_size, token = (uint32_t)slot - page * kv.page_size;
     const uint64_t at = (uint64_t)page * kv.page_stride + (uint64_t)token * kv.token_stride;
-    bool have_angles = false;
-    for (uint32_t u = blockIdx.y * blockDim.x + threadIdx.x;; u += gridDim.y * blockDim.x) {
-        const bool live = u < units;
-        uint32_t h = 0, oa = 0, ob = 0, w = 0;
-        float a[V], b[V];
-        const float* bias = nullptr;
-        if (live) {
-            h = u / per_head;
-            w = u - h * per_head;
-            const bool pair_halves = p.half_layout && w < rot_units && h < p.q_heads + kv.kv_heads;
-            oa = pair_halves ? w * V : 2u * w * V;
-            ob = pair_halves ? half + w * V : oa + V;
-            const TA* src;
-            if (h < p.q_heads) {
-                src = static_cast<const TA*>(p.q) + (uint64_t)row * p.q_stride + h * d;
-                bias = p.bq ? p.bq + h * d : nullptr;
-            } else if (h < p.q_heads + kv.kv_heads) {
-                src = static_cast<const TA*>(p.k) + (uint64_t)row * p.k_stride + (h - p.q_heads) * d;
-                bias = p.bk ? p.bk + (h - p.q_heads) * d : nullptr;
-            } else {
-                const uint32_t hv = h - p.q_heads - kv.kv_heads;
-                src = static_cast<const TA*>(p.v) + (uint64_t)row * p.v_stride + hv * d;
-                bias = p.bv ? p.bv + hv * d : nullptr;
-            }
-            load_vec<V>(src + oa, a);
-            load_vec<V>(src + ob, b);
-        }
-        if (!have_angles) {  // after the first loads have been sent
-            for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
-                const double turns = (double)pos * p.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
-                float s, c;
-                sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-                rope_smem[i] = make_float2(c * p.attn_scale, s * p.attn_scale);
-            }
-            __syncthreads();
-            have_angles = true;
-        }
-        if (!live) break;
-        if (bias) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) a[i] += bias[oa + i], b[i] += bias[ob + i];
-        }
-        if (w < rot_units && h < p.q_heads + kv.kv_heads) {
-            const float2* cs = rope_smem + w * V;
+    while (u < units) {
+        if (x.w < rot_units && x.head < rot_heads) {
+            const float2* cs = rope_smem + x.w * V;
             if (p.half_layout) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float x = a[i], y = b[i];
-                    a[i] = x * cs[i].x - y * cs[i].y;
-                    b[i] = x * cs[i].y + y * cs[i].x;
+                    const float a = x.a[i], b = x.b[i];
+                    x.a[i] = a * cs[i].x - b * cs[i].y;
+                    x.b[i] = a * cs[i].y + b * cs[i].x;
                 }
             } else {
                 float z[2 * V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) z[i] = a[i], z[V + i] = b[i];
+                for (int i = 0; i < V; ++i) z[i] = x.a[i], z[V + i] = x.b[i];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float x = z[2 * i], y = z[2 * i + 1];
-                    z[2 * i] = x * cs[i].x - y * cs[i].y;
-                    z[2 * i + 1] = x * cs[i].y + y * cs[i].x;
+                    const float a = z[2 * i], b = z[2 * i + 1];
+                    z[2 * i] = a * cs[i].x - b * cs[i].y;
+                    z[2 * i + 1] = a * cs[i].y + b * cs[i].x;
                 }
 #pragma unroll
-                for (int i = 0; i < V; ++i) a[i] = z[i], b[i] = z[V + i];
+                for (int i = 0; i < V; ++i) x.a[i] = z[i], x.b[i] = z[V + i];
             }
         }
         TC* dst;
-        if (h < p.q_heads)
-            dst = static_cast<TC*>(p.q_out) + (uint64_t)row * p.out_stride + h * d;
-        else if (h < p.q_heads + kv.kv_heads)
-            dst = static_cast<TC*>(kv.k_pages) + at + (uint64_t)(h - p.q_heads) * kv.head_stride;
+        if (x.head < p.q_heads)
+            dst = static_cast<TC*>(p.q_out) + (uint64_t)row * p.out_stride + x.head * d;
+        else if (x.head < rot_heads)
+            dst = static_cast<TC*>(kv.k_pages) + at + (uint64_t)(x.head - p.q_heads) * kv.head_stride;
         else
-            dst = static_cast<TC*>(kv.v_pages) + at + (uint64_t)(h - p.q_heads - kv.kv_heads) * kv.head_stride;
-        store_vec<V>(dst + oa, a);
-        store_vec<V>(dst + ob, b);
+            dst = static_cast<TC*>(kv.v_pages) + at + (uint64_t)(x.head - rot_heads) * kv.head_stride;
+        store_vec<V>(dst + x.oa, x.a);
+        store_vec<V>(dst + x.ob, x.b);
+        u += step;
+        if (u < units) load(u);
     }
 }
 
 template <typename TA, typename TC>
 cudaError_t launch_rope(const RopePaged& p, const arcllm_cuda_paged_kv& kv, bool vec, cudaStream_t stream) {
     const uint32_t units = (p.q_heads + 2u * kv.kv_heads) * (kv.head_dim / (vec ? 16u : 2u));
-    const uint32_t threads = std::min(256u, (units + 31u) / 32u * 32u);
-    // few rows: a CTA per 256 units, for latency; many: one CTA per row, so that its angles are made once
+    const uint32_t threads = std::min(kRopeThreads, (units + 31u) / 32u * 32u);
+    // few rows: a CTA per 512 units, for latency; many: one CTA per row, so that its angles are made once
     const uint32_t parts = p.rows <= 592u ? std::min(64u, (units + threads - 1u) / threads) : 1u;
     const dim3 grid(p.rows, parts);
     const size_t smem = (size_t)(p.rot_dim / 2u) * sizeof(float2);
@@ -426,7 +431,8 @@ int rope_kv_paged(int act_type, const RopePaged& p, const arcllm_cuda_paged_kv& 
     const bool vec = p.rot_dim % 16u == 0u && kv.head_dim % 16u == 0u && aligned16(p.q) && aligned16(p.k) &&
                      aligned16(p.v) && aligned16(p.q_out) && aligned16(kv.k_pages) && aligned16(kv.v_pages) &&
                      ((p.q_stride | p.k_stride | p.v_stride) * as) % 16u == 0u && p.out_stride % 8u == 0u &&
-                     kv.page_stride % 8u == 0u && kv.token_stride % 8u == 0u && kv.head_stride % 8u == 0u;
+                     kv.page_stride % 8u == 0u && kv.token_stride % 8u == 0u && kv.head_stride % 8u == 0u &&
+                     (!p.bq || aligned16(p.bq)) && (!p.bk || aligned16(p.bk)) && (!p.bv || aligned16(p.bv));
     const bool bf = kv.type == ARC_GGML_BF16;
     cudaError_t e;
     if (act_type == ARC_GGML_F32)
