@@ -168,22 +168,21 @@ struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
-template <int V, typename T>
-__device__ __forceinline__ void load_vec(const T* src, float (&x)[V]) {
-    if constexpr (V * sizeof(T) >= 16) {
-        constexpr int W = V * sizeof(T) / 16, E = 16 / sizeof(T);
-        uint4 w[W];
+template <typename T, int V>
+struct alignas(V * sizeof(T) >= 16 ? 16 : alignof(T)) Raw {  // V elements as they lie in memory
+    T v[V];
+    __device__ __forceinline__ void load(const T* src) {
+        if constexpr (V * sizeof(T) >= 16) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = reinterpret_cast<const uint4*>(src)[i];
+            for (uint32_t i = 0; i < V * sizeof(T) / 16; ++i)
+                reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-#pragma unroll
-            for (int j = 0; j < E; ++j) x[i * E + j] = Elem<T>::get(reinterpret_cast<const T*>(&w[i])[j]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = Elem<T>::get(src[i]);
+            for (int i = 0; i < V; ++i) v[i] = src[i];
+        }
     }
-}
+    __device__ __forceinline__ float operator[](int i) const { return Elem<T>::get(v[i]); }
+};
 
 template <int V, typename T>
 __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
@@ -198,109 +197,117 @@ __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
     }
 }
 
-// One CTA (part blockIdx.y of its units) per row.  A unit is 2V elements of
-// one head as two V-wide vectors: the two sides of V rotated pairs in the half
-// layout, 2V neighbours otherwise; it is read and written by one thread, so q
-// may be rotated in place.  Units of a head: rotated ones first.
+// A unit is 2V elements of one head as two V-wide vectors: the two sides of V
+// rotated pairs in the half layout, 2V neighbours otherwise; it is read and
+// written by one thread, so q may be rotated in place.  Units of a head: rotated
+// ones first.  An item is a unit for each thread of the CTA (part w % parts of row
+// w / parts); a CTA walks over items and reads the next one before it turns to
+// the current one, for which the angles are in shared memory after one barrier.
 // Angles pos * freq are formed and reduced to a fraction of a turn in 64 bits
 // (at 16384 an fp32 product is already 1e-3 off), then sin and cos in fp32.
-// The row is read before its slot and position are known, so that the loads are
-// on their way together (rows without a request are read for nothing).
 // Bounded by HBM traffic for many rows and by latency for few.
 constexpr uint32_t kRopeThreads = 512;
 template <typename TA, typename TC, int V>
 __global__ void __launch_bounds__(kRopeThreads) rope_kv_paged_kernel(RopePaged p, arcllm_cuda_paged_kv kv,
+                                                                     uint32_t parts, uint32_t items,
                                                                      unsigned int* err) {
     pdl_trigger();
     pdl_wait();  // q, k, v come from the preceding kernels
-    extern __shared__ float2 rope_smem[];  // (cos, sin) * attn_scale of the row's rot_dim / 2 pairs
-    const uint32_t row = blockIdx.x, d = kv.head_dim, half = p.rot_dim / 2u;
+    extern __shared__ float2 rope_smem[];  // (cos, sin) * attn_scale of rot_dim / 2 pairs, twice
+    const uint32_t d = kv.head_dim, half = p.rot_dim / 2u;
     const uint32_t per_head = d / (2u * V), rot_units = half / V, rot_heads = p.q_heads + kv.kv_heads;
-    const uint32_t units = (rot_heads + kv.kv_heads) * per_head, step = gridDim.y * blockDim.x;
-    struct Unit {
-        uint32_t head, oa, ob, w;  // head of q, k, v in a row; places of the vectors in it; number in the head
-        float a[V], b[V];
-        const float* bias;
-    } x;
-    auto load = [&](uint32_t u) {
-        x.head = u / per_head;
-        x.w = u - x.head * per_head;
-        const bool halves = p.half_layout && x.w < rot_units && x.head < rot_heads;
-        x.oa = halves ? x.w * V : 2u * x.w * V;
-        x.ob = halves ? half + x.w * V : x.oa + V;
-        const TA* src;
-        if (x.head < p.q_heads) {
-            src = static_cast<const TA*>(p.q) + (uint64_t)row * p.q_stride + x.head * d;
-            x.bias = p.bq ? p.bq + x.head * d : nullptr;
-        } else if (x.head < rot_heads) {
-            src = static_cast<const TA*>(p.k) + (uint64_t)row * p.k_stride + (x.head - p.q_heads) * d;
-            x.bias = p.bk ? p.bk + (x.head - p.q_heads) * d : nullptr;
-        } else {
-            src = static_cast<const TA*>(p.v) + (uint64_t)row * p.v_stride + (x.head - rot_heads) * d;
-            x.bias = p.bv ? p.bv + (x.head - rot_heads) * d : nullptr;
-        }
-        load_vec<V>(src + x.oa, x.a);
-        load_vec<V>(src + x.ob, x.b);
-        if (x.bias) {
-            float ba[V], bb[V];
-            load_vec<V>(x.bias + x.oa, ba);
-            load_vec<V>(x.bias + x.ob, bb);
-#pragma unroll
-            for (int i = 0; i < V; ++i) x.a[i] += ba[i], x.b[i] += bb[i];
-        }
+    const uint32_t units = (rot_heads + kv.kv_heads) * per_head;
+    struct Item {
+        uint32_t row, head, at, oa, ob;  // head of q, k, v in a row; its unit; places of the vectors in the head
+        int32_t slot, pos;
+        bool live, turned;
+        Raw<TA, V> a, b;
     };
-    uint32_t u = blockIdx.y * blockDim.x + threadIdx.x;
-    if (u < units) load(u);
-    const int32_t slot = p.slots[row], pos = p.positions[row];
-    if (slot < 0) return;  // a row without a request (uniform over the CTA)
-    if ((uint32_t)slot >= kv.n_pages * kv.page_size || pos < 0) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
-        return;
-    }
-    for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
-        const double turns = (double)pos * p.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        rope_smem[i] = make_float2(c * p.attn_scale, s * p.attn_scale);
-    }
-    __syncthreads();
-    const uint32_t page = (uint32_t)slot / kv.page_size, token = (uint32_t)slot - page * kv.page_size;
-    const uint64_t at = (uint64_t)page * kv.page_stride + (uint64_t)token * kv.token_stride;
-    while (u < units) {
-        if (x.w < rot_units && x.head < rot_heads) {
-            const float2* cs = rope_smem + x.w * V;
+    auto fetch = [&](uint32_t w, Item& x) {
+        x.row = w / parts;
+        const uint32_t u = (w - x.row * parts) * blockDim.x + threadIdx.x;
+        x.live = u < units;
+        x.slot = __ldg(p.slots + x.row);
+        x.pos = __ldg(p.positions + x.row);
+        x.head = u / per_head;
+        x.at = u - x.head * per_head;
+        x.turned = x.at < rot_units && x.head < rot_heads;
+        const bool halves = p.half_layout && x.turned;
+        x.oa = halves ? x.at * V : 2u * x.at * V;
+        x.ob = halves ? half + x.at * V : x.oa + V;
+        if (!x.live) return;
+        const TA* src = x.head < p.q_heads ? static_cast<const TA*>(p.q) + (uint64_t)x.row * p.q_stride + x.head * d
+                        : x.head < rot_heads
+                            ? static_cast<const TA*>(p.k) + (uint64_t)x.row * p.k_stride + (x.head - p.q_heads) * d
+                            : static_cast<const TA*>(p.v) + (uint64_t)x.row * p.v_stride + (x.head - rot_heads) * d;
+        x.a.load(src + x.oa);
+        x.b.load(src + x.ob);
+    };
+    Item next;
+    fetch(blockIdx.x, next);
+    float2* angles = rope_smem;
+    for (uint32_t w = blockIdx.x; w < items; w += gridDim.x) {
+        const Item x = next;
+        if (items - w > gridDim.x) fetch(w + gridDim.x, next);
+        if (x.slot < 0) continue;  // a row without a request (the same for all threads)
+        if ((uint32_t)x.slot >= kv.n_pages * kv.page_size || x.pos < 0) {
+            if (threadIdx.x == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
+            continue;
+        }
+        angles = angles == rope_smem ? rope_smem + half : rope_smem;  // others may still read the last item's
+        for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
+            const double turns = (double)x.pos * p.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
+            float s, c;
+            sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+            angles[i] = make_float2(c * p.attn_scale, s * p.attn_scale);
+        }
+        __syncthreads();
+        if (!x.live) continue;
+        const float* bias = x.head < p.q_heads ? p.bq : x.head < rot_heads ? p.bk : p.bv;
+        const uint32_t in_part = x.head < p.q_heads ? x.head : x.head < rot_heads ? x.head - p.q_heads : x.head - rot_heads;
+        float za[V], zb[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) za[i] = x.a[i], zb[i] = x.b[i];
+        if (bias) {
+            Raw<float, V> ba, bb;
+            ba.load(bias + in_part * d + x.oa);
+            bb.load(bias + in_part * d + x.ob);
+#pragma unroll
+            for (int i = 0; i < V; ++i) za[i] += ba[i], zb[i] += bb[i];
+        }
+        if (x.turned) {
+            const float2* cs = angles + x.at * V;
             if (p.half_layout) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float a = x.a[i], b = x.b[i];
-                    x.a[i] = a * cs[i].x - b * cs[i].y;
-                    x.b[i] = a * cs[i].y + b * cs[i].x;
+                    const float s = za[i], t = zb[i];
+                    za[i] = s * cs[i].x - t * cs[i].y;
+                    zb[i] = s * cs[i].y + t * cs[i].x;
                 }
             } else {
                 float z[2 * V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) z[i] = x.a[i], z[V + i] = x.b[i];
+                for (int i = 0; i < V; ++i) z[i] = za[i], z[V + i] = zb[i];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float a = z[2 * i], b = z[2 * i + 1];
-                    z[2 * i] = a * cs[i].x - b * cs[i].y;
-                    z[2 * i + 1] = a * cs[i].y + b * cs[i].x;
+                    const float s = z[2 * i], t = z[2 * i + 1];
+                    z[2 * i] = s * cs[i].x - t * cs[i].y;
+                    z[2 * i + 1] = s * cs[i].y + t * cs[i].x;
                 }
 #pragma unroll
-                for (int i = 0; i < V; ++i) x.a[i] = z[i], x.b[i] = z[V + i];
+                for (int i = 0; i < V; ++i) za[i] = z[i], zb[i] = z[V + i];
             }
         }
         TC* dst;
-        if (x.head < p.q_heads)
-            dst = static_cast<TC*>(p.q_out) + (uint64_t)row * p.out_stride + x.head * d;
-        else if (x.head < rot_heads)
-            dst = static_cast<TC*>(kv.k_pages) + at + (uint64_t)(x.head - p.q_heads) * kv.head_stride;
-        else
-            dst = static_cast<TC*>(kv.v_pages) + at + (uint64_t)(x.head - rot_heads) * kv.head_stride;
-        store_vec<V>(dst + x.oa, x.a);
-        store_vec<V>(dst + x.ob, x.b);
-        u += step;
-        if (u < units) load(u);
+        if (x.head < p.q_heads) {
+            dst = static_cast<TC*>(p.q_out) + (uint64_t)x.row * p.out_stride + x.head * d;
+        } else {
+            const uint32_t page = (uint32_t)x.slot / kv.page_size, token = (uint32_t)x.slot - page * kv.page_size;
+            dst = static_cast<TC*>(x.head < rot_heads ? kv.k_pages : kv.v_pages) + (uint64_t)page * kv.page_stride +
+                  (uint64_t)token * kv.token_stride + (uint64_t)in_part * kv.head_stride;
+        }
+        store_vec<V>(dst + x.oa, za);
+        store_vec<V>(dst + x.ob, zb);
     }
 }
 
@@ -308,14 +315,17 @@ template <typename TA, typename TC>
 cudaError_t launch_rope(const RopePaged& p, const arcllm_cuda_paged_kv& kv, bool vec, cudaStream_t stream) {
     const uint32_t units = (p.q_heads + 2u * kv.kv_heads) * (kv.head_dim / (vec ? 16u : 2u));
     const uint32_t threads = std::min(kRopeThreads, (units + 31u) / 32u * 32u);
-    // few rows: a CTA per 512 units, for latency; many: one CTA per row, so that its angles are made once
-    const uint32_t parts = p.rows <= 592u ? std::min(64u, (units + threads - 1u) / threads) : 1u;
-    const dim3 grid(p.rows, parts);
-    const size_t smem = (size_t)(p.rot_dim / 2u) * sizeof(float2);
-    if (vec)
-        return launch_kernel(rope_kv_paged_kernel<TA, TC, 8>, grid, dim3(threads), smem, stream, p, kv,
-                             dev_error_word());
-    return launch_kernel(rope_kv_paged_kernel<TA, TC, 1>, grid, dim3(threads), smem, stream, p, kv, dev_error_word());
+    const uint32_t parts = (units + threads - 1u) / threads;
+    const uint64_t items = (uint64_t)p.rows * parts;
+    if (items > 0x7fffffffull) return cudaErrorInvalidValue;
+    const size_t smem = (size_t)p.rot_dim * sizeof(float2);
+    auto go = [&](auto kernel) {
+        // as many CTAs as fit the card, each with its share of the items
+        const uint32_t fit = 148u * std::max(1u, 1024u / threads);
+        return launch_kernel(kernel, dim3((uint32_t)std::min<uint64_t>(items, fit)), dim3(threads), smem, stream, p, kv,
+                             parts, (uint32_t)items, dev_error_word());
+    };
+    return vec ? go(rope_kv_paged_kernel<TA, TC, 8>) : go(rope_kv_paged_kernel<TA, TC, 1>);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
