@@ -2,28 +2,27 @@
 // cores (B200, sm_100a).
 //
 // An item is one KV head and up to 2 x 128 packed rows ((row, head of the
-// group) pairs, whole rows); a unit is a tile of 128 positions.  Per item and
-// tile, for each half s of the rows:
+// group) pairs, whole rows); a unit is a tile of positions.  Per item and tile,
+// for each half s of the rows:
 //   S_s = Q_s K^T        tcgen05.mma, both operands in shared memory
 //   P_s = exp2(S_s - m)  one thread per row: S out of tensor memory, the row's
-//                        maximum and sum in registers, P back over S in 16 bits
+//                        maximum and sum in registers, P in 16 bits
 //   O_s += P_s V         tcgen05.mma, P in tensor memory, V in shared memory
-// The halves alternate: while one half's softmax runs, the tensor core works
-// on the other's products.
 //   warps 0..3, 4..7  softmax of half 0, 1, and its output
 //   warp 8            TMA: pages' K and V rows into a ring of tiles
-//   warps 9, 10       issue the MMAs of half 0, 1 in turn: one waits for its
-//                     operands while the other issues, and the turn keeps the
-//                     halves out of step (without it both softmaxes ran at once
-//                     and then both products: 4500 clocks a unit)
+//   warps 9, 10       issue the MMAs of half 0, 1
 //   warp 11           TMA: the next item's queries, as soon as the last S of the
 //                     item before is there
+// Tensor memory (512 columns of 128 rows) decides the tile: with O in 2 x D of
+// them, S and P of both halves fit side by side for 80 positions at D = 128 (at
+// D = 64 more; 96 is what a thread's registers hold).  With tiles of 128 at D = 128 P had to lie over S, S of the next
+// tile had to wait for the product, and the chain weights - products - S - softmax
+// of one half set the pace (3400 clocks for 128 positions); now S of the next tile
+// is formed as soon as a softmax has S in its registers.
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
-// last time (the sums carry the same factor, so the result is the same); MMAs
-// of one thread run in order, so when S of a tile is there, all products
-// before it are done and O may be touched, and P may lie over S.
-// K and V tiles are built from boxes of a power of two of positions that
-// divides the page, so tiles and pages need not match.
+// last time (the sums carry the same factor, so the result is the same).
+// K and V tiles are built from boxes of positions that divide the page and the
+// tile, so tiles and pages need not match.
 // All waits are bounded: on a timeout the roles leave their loops, drain what
 // they started and the error word is set.
 #include <algorithm>
@@ -36,21 +35,26 @@ namespace arc {
 namespace paged {
 namespace {
 
-constexpr uint32_t kTile = 128;  // positions
 constexpr uint32_t kThreads = 384;
-// Registers: the softmax threads hold a row of S.  (8 x 208 + 4 x 80) x 32 <= 384 x 168, what the block starts with.
-constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80;
 constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that is let pass
 
 template <int D>
 struct Layout {
+    static constexpr uint32_t kTile = D == 128 ? 80u : 96u;  // positions
+    static constexpr uint32_t kMaxBox = D == 128 ? 16u : 32u;  // positions of a copy: divides the tile
     static constexpr uint32_t kParts = D / 64;           // 64-dim parts: a row of one is 128 bytes
-    static constexpr uint32_t kGroup = kParts * 1024u;   // 8 rows: [part][8][128 bytes], as the pages' boxes arrive
-    static constexpr uint32_t kBytes = 16u * kGroup;     // a Q half, a K tile or a V tile: 128 rows
-    static constexpr uint32_t kStages = 4u * 128u / D;        // K and V tiles in the ring: 128 KB
+    static constexpr uint32_t kGroup = kParts * 1024u;   // 8 positions: [part][8][128 bytes], as the pages' boxes arrive
+    static constexpr uint32_t kBytes = kTile / 8u * kGroup;   // a K or V tile
+    static constexpr uint32_t kStages = D == 128 ? 6u : 10u;  // K and V tiles in the ring: 120 KB
     static constexpr uint32_t kQPart = 128u * 128u;      // Q: [part][128 rows][128 bytes]
-    static constexpr uint32_t kRing = 2u * kBytes;       // after the two Q halves
+    static constexpr uint32_t kQBytes = kParts * kQPart;
+    static constexpr uint32_t kRing = 2u * kQBytes;      // after the two Q halves
     static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
+    // columns of tensor memory of half s
+    static __device__ __forceinline__ uint32_t s_col(uint32_t s) { return s * kTile; }
+    static __device__ __forceinline__ uint32_t p_col(uint32_t s) { return 2u * kTile + s * (kTile / 2u); }
+    static __device__ __forceinline__ uint32_t o_col(uint32_t s) { return 512u - 2u * D + s * D; }
+    static_assert(3u * kTile <= 512u - 2u * D, "S and P of both halves beside O");
 };
 
 // An item costs about this many tiles beside its own (queries in, first S, last
@@ -60,6 +64,7 @@ constexpr uint32_t kItemCost = 2;
 
 // The item that a role is at, and the part of its tiles that this CTA does: of
 // the item's units [0, kItemCost + tiles), from v on, as many as are left.
+template <uint32_t T>
 struct Walk {
     uint32_t r, kvh, mt, v, left;
     uint32_t n_items;  // of the request
@@ -81,7 +86,7 @@ struct Walk {
         rows = min(per_item, q.n - first);
         lo = q.p0 + first;
         hi = lo + rows - 1u;
-        s = span_of<kTile>(a, lo, hi);
+        s = span_of<T>(a, lo, hi);
     }
     __device__ __forceinline__ uint32_t stop() const { return min(s.n + kItemCost, v + left); }
     __device__ __forceinline__ uint32_t begin() const { return max(v, kItemCost) - kItemCost; }
@@ -108,9 +113,10 @@ struct Walk {
     }
 };
 
+template <uint32_t T>
 __device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint32_t mt, uint32_t per_item) {
     const uint32_t first = mt * per_item, rows = min(per_item, q.n - first);
-    return kItemCost + span_of<kTile>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
+    return kItemCost + span_of<T>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
 }
 
 // A role's wait: false once any role has given up.  One vote decides for the
@@ -227,13 +233,16 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                            const __grid_constant__ CUtensorMap qmap, PageMap heads, Args a, uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
+                            const __grid_constant__ CUtensorMap qmap, PageMap heads, Args a,
+                            uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
                             unsigned int* err) {
     using L = Layout<D>;
+    constexpr uint32_t kTile = L::kTile;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
-    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], turn[2], done;
+    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2],
+        p_empty[2], o_full[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
@@ -244,9 +253,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&q_full[s], 1);
             mbar_init(&q_empty[s], 1);
             mbar_init(&s_full[s], 1);
+            mbar_init(&s_empty[s], 4);
             mbar_init(&p_full[s], 4);
+            mbar_init(&p_empty[s], 1);
             mbar_init(&o_full[s], 1);
-            mbar_init(&turn[s], 1);
         }
         mbar_init(&done, 2);
         abort_flag = 0;
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (load_req(a, r, q, any_bad) && q.n * a.gq > kRowMax) {
             const uint32_t items = (q.n + per_item - 1u) / per_item;
             if (items <= kAlone) {
-                for (uint32_t mt = 0; mt < items; ++mt) u += item_units(a, q, mt, per_item);
+                for (uint32_t mt = 0; mt < items; ++mt) u += item_units<kTile>(a, q, mt, per_item);
                 u = min(u * a.kv_heads, 0xfffffffeull);
             } else {
                 u = kMany;
@@ -285,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         load_req(a, r, q, bad);
         const uint32_t items = (q.n + per_item - 1u) / per_item;
         unsigned long long u = 0;
-        for (uint32_t mt = lane; mt < items; mt += 32u) u += item_units(a, q, mt, per_item);
+        for (uint32_t mt = lane; mt < items; mt += 32u) u += item_units<kTile>(a, q, mt, per_item);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         if (lane == 0) off[r + 1] = (uint32_t)min(u * a.kv_heads, 0xfffffffeull);
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t rem = U0 - off[r] - kvh * head, mt = 0;
         const uint32_t items = (q.n + per_item - 1u) / per_item;
         for (uint32_t m0 = 0; m0 < items; m0 += 32u) {  // the item that unit rem of the head lies in
-            uint32_t v = m0 + lane < items ? item_units(a, q, m0 + lane, per_item) : 0u;
+            uint32_t v = m0 + lane < items ? item_units<kTile>(a, q, m0 + lane, per_item) : 0u;
             const uint32_t mine = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -331,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
-    Walk w;
+    Walk<kTile> w;
     bool any = n_units != 0;
     if (any) {
         w.r = __shfl_sync(0xffffffffu, start[0], 0), w.kvh = __shfl_sync(0xffffffffu, start[1], 0);
@@ -342,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (w.begin() == w.end()) any = w.next(a, off, per_item);
     }
     if (warp >= 8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       if (!any) {
         // nothing to do; the tensor memory is given back below
       } else if (warp == 8) {
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool bad_page = false, ok = true;
         // lane b: box b of a tile; it is loaded when it holds anything that is seen
         uint32_t i = w.begin(), end = w.end();
-        auto entry = [&](const Walk& x) -> int {
+        auto entry = [&](const Walk<kTile>& x) -> int {
             const uint32_t p = x.s.tile(i) * kTile + lane * box;
             const uint32_t from = a.window && x.lo >= a.window ? x.lo - a.window + 1u : 0u;
             if (lane >= boxes || p > x.hi || (p + box <= from && p >= a.sinks)) return -1;
@@ -393,62 +402,57 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
       } else if (warp < 11) {
         // ---------------- MMA of half s ----------------
-        constexpr uint32_t kQk = instr_desc<BF16>(128, false), kPv = instr_desc<BF16>(D, true);
-        const uint32_t s = warp - 9u, leader = lane == 0;
-        const uint32_t ring = smem_addr(smem + L::kRing), ts = tmem + s * 128u, to = tmem + 256u + s * 128u;
-        const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kBytes, 16u, 1024u);
-        uint32_t stage = 0, phase = 0, n_item = 0, n_p = 0, n_turn = s ^ 1u;
+        constexpr uint32_t kQk = instr_desc<BF16>(kTile, false), kPv = instr_desc<BF16>(D, true);
+        const uint32_t s = warp - 9u, leader = lane == 0, ring = smem_addr(smem + L::kRing);
+        const uint32_t ts = tmem + L::s_col(s), tp = tmem + L::p_col(s), to = tmem + L::o_col(s);
+        const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kQBytes, 16u, 1024u);
+        // Tiles come as K, V, K, V ...; K of the next one is used before V of this one.
+        struct At {
+            uint32_t stage, phase;
+            __device__ __forceinline__ void advance() {
+                stage += 2u;
+                if (stage >= L::kStages) stage -= L::kStages, phase ^= 1u;
+            }
+        } at_k{0, 0}, at_v{1, 0};
+        uint32_t n_item = 0, n_s = 0, n_p = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = role_wait(bar, parity, &abort_flag, err); };
-        auto my_turn = [&]() {  // half 0 begins
-            const bool got = wait(&turn[s], n_turn++ & 1u);
-            tmem_fence_after();
-            return got;
-        };
-        auto pass_turn = [&]() {
-            if (leader) mbar_arrive(&turn[s ^ 1u]);
-        };
-        auto advance = [&]() {
-            if (++stage == L::kStages) stage = 0, phase ^= 1u;
-        };
-        auto qk = [&](uint32_t k_stage) {  // S = Q K^T
-            const uint64_t kb = operand_desc(ring + k_stage * L::kBytes, 16u, L::kGroup);
+        auto qk = [&](bool live) {  // S = Q K^T of the tile at at_k, once the softmax has the last S
+            if (!wait(&kv_full[at_k.stage], at_k.phase)) return false;
+            if (live) {
+                if (n_s != 0u && !wait(&s_empty[s], (n_s - 1u) & 1u)) return false;
+                ++n_s;
+                tmem_fence_after();
+                const uint64_t kb = operand_desc(ring + at_k.stage * L::kBytes, 16u, L::kGroup);
 #pragma unroll
-            for (uint32_t kk = 0; kk < D / 16u; ++kk) {
-                // addresses count 16 bytes
-                mma_smem(ts, qa + (((kk >> 2) * L::kQPart + (kk & 3u) * 32u) >> 4),
-                         kb + (((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4), kQk, kk != 0u, leader);
+                for (uint32_t kk = 0; kk < D / 16u; ++kk)  // addresses count 16 bytes
+                    mma_smem(ts, qa + (((kk >> 2) * L::kQPart + (kk & 3u) * 32u) >> 4),
+                             kb + (((kk >> 2) * 1024u + (kk & 3u) * 32u) >> 4), kQk, kk != 0u, leader);
+                mma_commit(&s_full[s], leader);
             }
-            mma_commit(&s_full[s], leader);
+            mma_commit(&kv_empty[at_k.stage], leader);
+            at_k.advance();
+            return true;
         };
         do {
             const uint32_t i0 = w.begin(), i1 = w.end();
-            const bool live = s == 0u || w.rows > half_rows;  // otherwise the half only passes its turns on
-            if (!wait(&kv_full[stage], phase)) break;
+            const bool live = s == 0u || w.rows > half_rows;  // otherwise the tiles pass by
             if (live && !wait(&q_full[s], n_item++ & 1u)) break;
-            if (!my_turn()) break;
-            if (live) qk(stage);
-            pass_turn();
-            if (live && i1 - i0 == 1u) mma_commit(&q_empty[s], leader);
-            mma_commit(&kv_empty[stage], leader);
-            advance();
+            if (!qk(live)) break;
+            if (live && i0 + 1u == i1) mma_commit(&q_empty[s], leader);
             for (uint32_t i = i0; i < i1; ++i) {
-                const uint32_t v_stage = stage;
-                const bool more = i + 1u < i1;
-                if (!wait(&kv_full[v_stage], phase)) break;
-                advance();
-                const uint32_t k_stage = stage;
-                if (more) {  // the next K too: nothing is waited for between the products
-                    if (!wait(&kv_full[k_stage], phase)) break;
-                    advance();
+                if (i + 1u < i1) {
+                    if (!qk(live)) break;
+                    if (live && i + 2u == i1) mma_commit(&q_empty[s], leader);  // that was the last S
                 }
+                if (!wait(&kv_full[at_v.stage], at_v.phase)) break;
                 // V rows of positions that no row of the item sees are zeroed (by both warps): what lies there may be
                 // anything, and the weight 0 does not stop a NaN.
                 const uint32_t p0 = w.s.tile(i) * kTile;
                 const uint32_t from = a.window && w.lo >= a.window ? w.lo - a.window + 1u : 0u;
                 const bool tail = p0 + kTile - 1u > w.hi, gap = p0 < from && p0 + kTile > a.sinks;
                 if (tail || gap) {
-                    uint8_t* v = smem + L::kRing + v_stage * L::kBytes + (lane & 7u) * 16u;
+                    uint8_t* v = smem + L::kRing + at_v.stage * L::kBytes + (lane & 7u) * 16u;
                     auto clear = [&](uint32_t r0, uint32_t r1) {  // rows [r0, r1): 8 lanes a row of 128 bytes
 #pragma unroll 2
                         for (uint32_t r = r0 + (lane >> 3); r < r1; r += 4u)
@@ -462,22 +466,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                if (live && !wait(&p_full[s], n_p++ & 1u)) break;
-                if (!my_turn()) break;
                 if (live) {
-                    const uint64_t vb = operand_desc(ring + v_stage * L::kBytes, 1024u, L::kGroup);
+                    if (!wait(&p_full[s], n_p++ & 1u)) break;
+                    tmem_fence_after();
+                    const uint64_t vb = operand_desc(ring + at_v.stage * L::kBytes, 1024u, L::kGroup);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
-                        mma_tmem(to, ts + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv, i != i0 || kk != 0u, leader);
-                    if (more)
-                        qk(k_stage);
-                    else
-                        mma_commit(&o_full[s], leader);
+                        mma_tmem(to, tp + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv, i != i0 || kk != 0u, leader);
+                    mma_commit(&p_empty[s], leader);
+                    if (i + 1u == i1) mma_commit(&o_full[s], leader);
                 }
-                pass_turn();
-                if (live && i + 2u == i1) mma_commit(&q_empty[s], leader);  // the last S has been issued
-                mma_commit(&kv_empty[v_stage], leader);
-                if (more) mma_commit(&kv_empty[k_stage], leader);
+                mma_commit(&kv_empty[at_v.stage], leader);
+                at_v.advance();
             }
         } while (ok && w.next(a, off, per_item));
         if (!ok) abort_flag = 1;
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive_expect_tx(&q_full[s], L::kParts * half_rows * a.gq * 128u);
 #pragma unroll
                     for (uint32_t c = 0; c < L::kParts; ++c)
-                        tma_queries(smem + s * L::kBytes + c * L::kQPart, &qmap, (int)c, (int)(w.kvh * a.gq),
+                        tma_queries(smem + s * L::kQBytes + c * L::kQPart, &qmap, (int)c, (int)(w.kvh * a.gq),
                                     (int)(w.q.row0 + w.first + s * half_rows), &q_full[s]);
                 }
                 __syncwarp();
@@ -511,13 +511,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n[s] != 0u) mbar_wait(&q_full[s], (n[s] - 1u) & 1u, err);
       }
     } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       if (any) {
         // ---------------- softmax of half s: thread t has packed row t ----------------
         const uint32_t s = warp >> 2, t = tid & 127u;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
-        const uint32_t ts = tmem + lanes + s * 128u, to = tmem + lanes + 256u + s * 128u;
-        uint32_t n_s = 0, n_o = 0;
+        const uint32_t ts = tmem + lanes + L::s_col(s), tp = tmem + lanes + L::p_col(s), to = tmem + lanes + L::o_col(s);
+        uint32_t n_s = 0, n_o = 0;  // tiles, items so far
         const uint32_t t_row = t / a.gq;
         bool ok = true;
         for (bool more = true; more;) {
@@ -534,44 +533,46 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (uint32_t i = i0; i < i1; ++i) {
                 ok = role_wait(&s_full[s], n_s & 1u, &abort_flag, err);
                 if (!ok) break;
-                ++n_s;
                 tmem_fence_after();
+                float x[kTile];
+                tmem_ld(ts, x);
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty[s]);  // the next S may come
                 const uint32_t p0 = w.s.tile(i) * kTile;
                 // not all rows see all of it: behind a row's position, before its window and past the sinks
                 const bool past = p0 + kTile - 1u > p_lo;
                 const bool before = a.window && p0 + a.window <= p_hi && p0 + kTile > a.sinks;
-                const int last = (int)(pos - p0);
-                int first = 0, sinks = 0;
-                if (before && pos + 1u >= a.window) first = (int)(pos + 1u - a.window - p0), sinks = (int)(a.sinks - p0);
-                // 64 columns at a time in a loop that stays one: tensor memory gives 128 columns in 90 clocks, so S is
-                // read twice rather than kept in 128 registers, and the code of all roles stays small enough for the
-                // instruction caches, which straight-line code for 128 columns was not.
-                float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-                for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
-                    float x[64];
-                    tmem_ld64(ts + c0, x);
-                    if (past || before) {  // -inf where the row does not see, also for the second reading
-                        const int e = last - (int)c0, f = first - (int)c0, g = sinks - (int)c0;
-                        if (before) {
+                if (past || before) {
+                    const int last = (int)(pos - p0);
+                    if (before) {
+                        int first = 0, sinks = 0;
+                        if (pos + 1u >= a.window) first = (int)(pos + 1u - a.window - p0), sinks = (int)(a.sinks - p0);
 #pragma unroll
-                            for (int c = 0; c < 64; ++c)
-                                if (c < f && c >= g) x[c] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c > e) x[c] = -INFINITY;
-                        tmem_st64(ts + c0, x);
+                        for (int c = 0; c < (int)kTile; ++c)
+                            if (c < first && c >= sinks) x[c] = -INFINITY;
                     }
 #pragma unroll
-                    for (uint32_t c = 0; c < 64u; c += 4u)
-#pragma unroll
-                        for (uint32_t k = 0; k < 2u; ++k) mx[k] = max_nan(mx[k], x[c + 2u * k], x[c + 2u * k + 1u]);
+                    for (int c = 0; c < (int)kTile; ++c)
+                        if (c > last) x[c] = -INFINITY;
                 }
-                if (past || before) tmem_wait_st();
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (uint32_t c = 4; c + 8u <= kTile; c += 8u)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k) mx[k] = max_nan(mx[k], x[c + k], x[c + 4u + k]);
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) mx[k] = max_nan(mx[k], x[kTile - 4u + k]);
                 // An infinite score has no softmax: NaN for the row, as for a NaN score.
-                float mn = max_nan(mx[0], mx[1]) * a.scale_log2;
+                float mn = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale_log2;
                 if (mn == INFINITY) mn = NAN;
+                bool waited = n_s == 0u;  // for the product before: P's columns, and O
+                auto product = [&]() {
+                    if (!waited) ok = role_wait(&p_empty[s], (n_s - 1u) & 1u, &abort_flag, err);
+                    waited = true;
+                    tmem_fence_after();
+                    return ok;
+                };
                 if (i == i0) {
                     m = mn;  // O is written afresh
                 } else if (__any_sync(0xffffffffu, live && !(mn <= m + kGrow))) {
@@ -579,27 +580,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float f = ex2(m - (to_m == -INFINITY ? 0.f : to_m));
                     l *= f;
                     m = to_m;
+                    if (!product()) break;
 #pragma unroll 1
                     for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
                         float o[32];
-                        tmem_ld32(to + c, o);
+                        tmem_ld(to + c, o);
                         uint32_t ob[32];
 #pragma unroll
                         for (uint32_t k = 0; k < 32u; ++k) ob[k] = __float_as_uint(o[k] * f);
-                        tmem_st32(to + c, ob);
+                        tmem_st(to + c, ob);
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
                 uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll 1
-                for (uint32_t c0 = 0; c0 < kTile; c0 += 64u) {
-                    float x[64];
-                    tmem_ld64(ts + c0, x);
-                    uint32_t pk[32];
+                constexpr uint32_t kAtOnce = kTile == 80u ? 80u : 32u;  // columns between two stores
 #pragma unroll
-                    for (uint32_t c = 0; c < 64u; c += 2u) {
-                        const uint64_t y2 = fma2(pair(x[c], x[c + 1u]), c2, r2);
+                for (uint32_t c0 = 0; c0 < kTile; c0 += kAtOnce) {
+                    uint32_t pk[kAtOnce / 2u];
+#pragma unroll
+                    for (uint32_t c = 0; c < kAtOnce; c += 2u) {
+                        const uint64_t y2 = fma2(pair(x[c0 + c], x[c0 + c + 1u]), c2, r2);
                         float2 e;
                         if (c % 8u == 6u) {
                             e = exp2_poly<BF16>(y2);
@@ -611,10 +612,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // the product takes weights of the cache's type: half a step of it each, as the output
                         pk[c / 2u] = pack16<BF16>(e.x, e.y);
                     }
-                    tmem_st32(ts + c0 / 2u, pk);  // over columns that have been read
+                    if (c0 == 0u && !product()) break;
+                    tmem_st(tp + c0 / 2u, pk);
                 }
+                if (!ok) break;
                 const float2 sm = unpair(add2(sum[0], sum[1]));
                 l += sm.x + sm.y;
+                ++n_s;
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
@@ -641,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (uint32_t c = 0; c < (uint32_t)D; c += 32u) {
                 float o[32];
-                tmem_ld32(to + c, o);
+                tmem_ld(to + c, o);
                 if (whole) {
                     // 16 bytes of each of four neighbours' rows instead of 64 of its own: a store then touches 8 rows
                     // of 64 bytes rather than 32 of 16
@@ -686,8 +690,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int D, bool BF16>
 int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, float* parts, cudaStream_t stream) {
     using L = Layout<D>;
-    uint32_t box = 16;  // the largest power of two up to the tile that divides the page
-    while (box < kTile && kv.page_size % (2u * box) == 0u) box *= 2u;
+    uint32_t box = 16;  // the largest power of two that divides the page, and the tile
+    while (box < L::kMaxBox && kv.page_size % (2u * box) == 0u) box *= 2u;
     CUtensorMap kmap, vmap;
     PageMap heads;
     const int st = encode_pages(&kmap, &vmap, &heads, kv, box);
