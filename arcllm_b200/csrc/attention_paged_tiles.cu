@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // not all rows see all of it: behind a row's position, before its window and past the sinks
                 const bool past = p0 + kTile - 1u > p_lo;
                 const bool before = a.window && p0 + a.window <= p_hi && p0 + kTile > a.sinks;
-                if (past || before) {
+                if (__builtin_expect(past || before, 0)) {
                     const int last = (int)(pos - p0);
                     if (before) {
                         int first = 0, sinks = 0;
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 if (i == i0) {
                     m = mn;  // O is written afresh
-                } else if (__any_sync(0xffffffffu, live && !(mn <= m + kGrow))) {
+                } else if (__builtin_expect(__any_sync(0xffffffffu, live && !(mn <= m + kGrow)), 0)) {
                     const float to_m = max_nan(m, mn);
                     const float f = ex2(m - (to_m == -INFINITY ? 0.f : to_m));
                     l *= f;
