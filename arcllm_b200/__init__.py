@@ -153,7 +153,8 @@ def check(status, what=""):
 
 def call(name, *args):
     """Invoke an entry point and raise ArcError on a non-zero status."""
-    return check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)  # the lock only until the library is there
+    return check(status, name) if status else status
 
 
 class ModelConfig(C.Structure):

@@ -366,7 +366,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 
 // ---- join ---------------------------------------------------------------------
 // Block (c, part): the item that CTA c began and later CTAs went on with.  The
-// first kSms records are the rows kernel's, the others the tile kernel's.
+// first kSms records are the rows kernel's, the others the tile kernel's.  Nearly
+// always two CTAs share an item: then a thread has four pairs of loads on their
+// way; a longer row of parts is walked eight at a time.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Record* __restrict__ recs,
                                                               const float* __restrict__ row_parts,
@@ -378,21 +380,57 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Reco
     const bool tiles = rec0 + blockIdx.x >= kSms;
     const uint32_t cta = rec0 + blockIdx.x - (tiles ? kSms : 0u);
     const uint32_t max_rows = tiles ? kTileRows : kRowMax, stride = max_rows * (D + 2u);
-    const float* parts = tiles ? tile_parts : row_parts;
-    for (uint32_t x = blockIdx.y * blockDim.x + threadIdx.x; x < rc.rows * (D / 4u); x += gridDim.y * blockDim.x) {
-        const uint32_t ri = x / (D / 4u), c = (x - ri * (D / 4u)) * 4u;
+    const float* first = (tiles ? tile_parts : row_parts) + (uint64_t)(cta * 2u + 1u) * stride;
+    const float* later = first + stride;  // slot 0 of the next CTA; those after it 2 * stride apart
+    const uint32_t n = rc.last_cta - cta, total = rc.rows * (D / 4u);
+    auto write = [&](uint32_t ri, uint32_t c, float4 A, float L) {
+        const uint32_t qr = ri / a.gq;
+        const float inv = 1.f / L;
+        *reinterpret_cast<uint2*>(a.out + (uint64_t)(rc.row0 + qr) * a.out_stride +
+                                  (rc.kvh * a.gq + ri - qr * a.gq) * D + c) =
+            make_uint2(pack16<BF16>(A.x * inv, A.y * inv), pack16<BF16>(A.z * inv, A.w * inv));
+    };
+    const uint32_t step = gridDim.y * 256u;
+    if (n == 1u) {
+        constexpr uint32_t U = 4;
+        for (uint32_t x0 = blockIdx.y * 256u + threadIdx.x; x0 < total; x0 += U * step) {
+            float4 v[U], y[U];
+            float2 mv[U], my[U];
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                const uint32_t x = min(x0 + j * step, total - 1u), ri = x / (D / 4u);
+                v[j] = reinterpret_cast<const float4*>(first)[x];
+                y[j] = reinterpret_cast<const float4*>(later)[x];
+                mv[j] = *reinterpret_cast<const float2*>(first + max_rows * D + 2u * ri);
+                my[j] = *reinterpret_cast<const float2*>(later + max_rows * D + 2u * ri);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                const uint32_t x = x0 + j * step;
+                if (x >= total) break;
+                const float M = fmaxf(mv[j].x, my[j].x), f = ex2(mv[j].x - M), g = ex2(my[j].x - M);
+                write(x / (D / 4u), x % (D / 4u) * 4u,
+                      make_float4(fmaf(v[j].x, f, y[j].x * g), fmaf(v[j].y, f, y[j].y * g),
+                                  fmaf(v[j].z, f, y[j].z * g), fmaf(v[j].w, f, y[j].w * g)),
+                      fmaf(mv[j].y, f, my[j].y * g));
+            }
+        }
+        return;
+    }
+    for (uint32_t x = blockIdx.y * 256u + threadIdx.x; x < total; x += step) {
+        const uint32_t ri = x / (D / 4u), c = x % (D / 4u) * 4u;
         constexpr uint32_t CH = 8;  // parts whose loads are in flight together
         float M = -INFINITY, L = 0.f;
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t j0 = cta; j0 <= rc.last_cta; j0 += CH) {
+        for (uint32_t j0 = 0; j0 <= n; j0 += CH) {
             float2 ml[CH];
             float4 v[CH];
 #pragma unroll
             for (uint32_t j = 0; j < CH; ++j) {
                 ml[j] = make_float2(-INFINITY, 0.f);
                 v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (j0 + j <= rc.last_cta) {
-                    const float* p = parts + (uint64_t)((j0 + j) * 2u + (j0 + j == cta ? 1u : 0u)) * stride;
+                if (j0 + j <= n) {
+                    const float* p = j0 + j == 0u ? first : later + (uint64_t)(j0 + j - 1u) * 2u * stride;
                     ml[j] = *reinterpret_cast<const float2*>(p + max_rows * D + 2u * ri);
                     v[j] = *reinterpret_cast<const float4*>(p + ri * D + c);
                 }
@@ -412,11 +450,7 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(Args a, const Reco
             }
             M = mn;
         }
-        const uint32_t qr = ri / a.gq;
-        const float inv = 1.f / L;
-        *reinterpret_cast<uint2*>(a.out + (uint64_t)(rc.row0 + qr) * a.out_stride +
-                                  (rc.kvh * a.gq + ri - qr * a.gq) * D + c) =
-            make_uint2(pack16<BF16>(A.x * inv, A.y * inv), pack16<BF16>(A.z * inv, A.w * inv));
+        write(ri, c, A, L);
     }
 }
 
@@ -443,8 +477,7 @@ int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args&
         const uint32_t slot_rows = !many && a.max_new * a.gq <= 8u ? 8u : 16u;
         const uint32_t fixed = 1024u + kRowWarps * slot_rows * (D + 2u) * 4u + 4u * (a.n_requests + 1u);
         const uint32_t stages = std::min(4u, (kMost - fixed) / (kRowWarps * kStage));
-        e = cudaFuncSetAttribute(attn_paged_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)kMost);
+        e = allow_shared<attn_paged_rows_kernel<D, BF16>>((int)kMost);
         if (e == cudaSuccess)
             e = launch_kernel(attn_paged_rows_kernel<D, BF16>, dim3(kSms), dim3(kRowWarps * 32u),
                               fixed + kRowWarps * stages * kStage, stream, kmap, vmap, heads, a, slot_rows, stages, recs,
@@ -456,7 +489,7 @@ int launch_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, const Args&
     }
     // blocks of the records that were written
     if (e == cudaSuccess)
-        e = launch_kernel(attn_paged_join_kernel<D, BF16>, dim3((few ? kSms : 0u) + (many ? kSms : 0u), many ? 16 : 2),
+        e = launch_kernel(attn_paged_join_kernel<D, BF16>, dim3((few ? kSms : 0u) + (many ? kSms : 0u), many ? 4 : 2),
                           dim3(256), 0, stream, a, recs, parts, tile_parts, few ? 0u : kSms);
     return launch_checked(e, "attention paged launch");
 }

@@ -709,8 +709,7 @@ int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, fl
         if (rc != CUDA_SUCCESS) return set_error(ARC_E_CUDA, "attention paged: tensor map of the queries");
     }
     const uint32_t smem = 1024u + L::kOff + 4u * (a.n_requests + 1u);
-    cudaError_t e = cudaFuncSetAttribute(attn_paged_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
+    cudaError_t e = allow_shared<attn_paged_tiles_kernel<D, BF16>>((int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
     if (e == cudaSuccess)
         e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap,
                           qmap, heads, a, box, 1u, recs, parts, dev_error_word());

@@ -347,10 +347,7 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
     const uint32_t smem = counts || p.bias_start
                               ? (chunk + 31u) / 32u * 8u + 4u + 4u * kList + 4u * kNamed * (p.bias_start ? 2u : 1u)
                               : 0u;
-    cudaError_t e = cudaFuncSetAttribute(logits_process_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(logits_process_kernel<T, V>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = allow_shared<logits_process_kernel<T, V>, true>(kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
     if (e != cudaSuccess) return e;
     LogitsProcess q = p;
     q.n_rows = rows;

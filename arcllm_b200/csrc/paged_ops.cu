@@ -358,8 +358,7 @@ int paged_plan(const PagedPlan& p, cudaStream_t stream) {
             return set_error(ARC_E_INVALID_ARGUMENT, "paged plan: an output overlaps an input");
     const uint32_t smem = 12u * p.n_requests;
     if (smem > 48u * 1024u - 1024u) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 12 * kPlanMaxRequests);
+        const cudaError_t e = allow_shared<paged_plan_kernel>(12 * kPlanMaxRequests);
         if (e != cudaSuccess) return set_cuda_error(e, "paged plan");
     }
     const uint32_t grid = std::min(148u, (p.max_rows + 4u * kPlanThreads - 1u) / (4u * kPlanThreads));

@@ -3,11 +3,27 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
-#include "../../include/arcllm_cuda.h"
+#include "arcllm_cuda_internal.h"
 
 namespace arc {
+
+// The kernel's limit of dynamic shared memory (and, if asked, clusters of 16) on
+// the current device, set once for each device: the attribute calls cost a
+// microsecond of every launch otherwise.
+template <auto Kernel, bool kClusters16 = false>
+cudaError_t allow_shared(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    const int dev = device_slot();
+    if (dev >= 0 && ((done.load(std::memory_order_acquire) >> dev) & 1u)) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && kClusters16)
+        e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev >= 0) done.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+}
 
 struct PagedPlan {
     const int32_t *kv_len, *new_len;
