@@ -555,6 +555,8 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: heads side by side in a token, or one after another");
     if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31))
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: a stride past 2^40 bytes");
+    if (rows_meet(p.q, p.q_stride, p.out, p.out_stride, p.max_rows, width, 2u))
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: out overlaps q");
     if (p.workspace_bytes < need) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: workspace too small");
     Args a{};
     a.q = static_cast<const uint16_t*>(p.q);
@@ -565,7 +567,8 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
     a.n_requests = p.n_requests, a.max_rows = p.max_rows, a.max_new = p.max_new;
     a.kv_heads = kv.kv_heads, a.gq = gq, a.page_size = kv.page_size, a.n_pages = kv.n_pages;
     a.scale_log2 = (float)((double)p.scale * 1.4426950408889634074);
-    a.window = p.window, a.sinks = p.window ? p.sinks : 0u;
+    a.window = std::min(p.window, 0x7fffffffu);  // positions are below 2^31: sums stay within 32 bits
+    a.sinks = p.window ? std::min(p.sinks, 0x7fffffffu) : 0u;
     const bool bf = kv.type == ARC_GGML_BF16;
     if (kv.head_dim == 128u)
         return bf ? launch_paged<128, true>(p, kv, a, stream) : launch_paged<128, false>(p, kv, a, stream);

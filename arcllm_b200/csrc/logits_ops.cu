@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
     const uint32_t v_begin = min(blockIdx.x * slice, p.vocab), v_end = min(v_begin + slice, p.vocab);
     const T* in = static_cast<const T*>(p.logits) + (uint64_t)row * p.stride;
     T* out = static_cast<T*>(p.out) + (uint64_t)row * p.out_stride;
-    constexpr uint32_t U = 4;  // vectors in flight per thread
+    constexpr uint32_t U = V > 1 ? 4 : 16;  // vectors, or single values, in flight per thread
     T x[U][V];
     auto load = [&](uint32_t i0, uint32_t i1) {  // of the part's tokens [i0, i1)
 #pragma unroll

@@ -69,6 +69,18 @@ struct LogitsProcess {
 };
 int logits_process(int type, const LogitsProcess& p, cudaStream_t stream);
 
+// Whether two arrays of rows of `width` elements of `size` bytes share a byte.  Rows of one stride may lie side by
+// side in one array (parts of a fused projection); with different strides any overlap of the whole ranges counts.
+inline bool rows_meet(const void* a, uint64_t a_stride, const void* b, uint64_t b_stride, uint64_t rows,
+                      uint64_t width, uint64_t size) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const uint64_t na = ((rows - 1u) * a_stride + width) * size, nb = ((rows - 1u) * b_stride + width) * size;
+    if (x >= y + nb || y >= x + na) return false;
+    if (a_stride != b_stride) return true;
+    const uint64_t off = (x > y ? x - y : y - x) % (a_stride * size);
+    return off < width * size || a_stride * size - off < width * size;
+}
+
 // Checks of a cache descriptor that every user of it makes (null pointers, shape, type, the 32-bit slot range).
 int check_paged_kv(const arcllm_cuda_paged_kv* kv, const char* who);
 

@@ -472,7 +472,8 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  * p = kv_total[r] - n + i, n its number of rows, and sees positions j <= p;
  * with window > 0 only those with j > p - window or j < sinks.
  *   q, out       [max_rows][q_heads*head_dim] of the cache's type, row strides
- *                in elements; rows of no request are left as they were;
+ *                in elements, apart from one another; rows of no request are
+ *                left as they were;
  *   block_table  as arcllm_cuda_paged_plan leaves it; entries of pages that no
  *                row sees (before the window) are not read as pages' numbers;
  *   max_new      at least the largest number of rows of one request;

@@ -67,6 +67,12 @@ def test_rope_refusals():
         assert status(f, changed(good, 18, kv(**k))) == want, k
     assert status(f, changed(good, 18, kv(head_dim=5, token_stride=5, head_stride=5))) == INVALID
     assert status(f, changed(good, 16, 0)) == b"ARC_OK"
+    same = changed(good, 19, a[0])  # in place, but fp32 q into fp16
+    assert status(f, same) == INVALID
+    half = changed(same, 0, A.GGML_F16)
+    assert status(f, changed(half, 20, 520)) == INVALID  # other rows
+    assert status(f, changed(changed(good, 0, A.GGML_F16), 19, P((3 << 20) + 1000))) == INVALID  # half a row on
+    assert status(f, changed(good, 19, P((3 << 20) + 2048))) == INVALID  # row 1 of q
 
 
 def test_attention_refusals():
@@ -90,6 +96,9 @@ def test_attention_refusals():
     assert status(f, changed(changed(changed(good, 10, 129), 1, 129 * 128), 15, 129 * 128)) == SHAPE  # heads a group
     for i in (7, 8, 9):
         assert status(f, changed(good, i, 0)) == b"ARC_OK", i  # nothing to do
+    assert status(f, changed(good, 14, a[0])) == INVALID  # out is q
+    assert status(f, changed(good, 14, P((3 << 20) + 1024 + 512))) == INVALID  # between its rows
+    assert status(f, changed(changed(good, 14, P((3 << 20) + 1024)), 15, 520)) == INVALID
 
 
 def test_attention_workspace():

@@ -181,7 +181,8 @@ def test_attention_few_rows(name, dim, heads, gq, page, heads_first):
 
 
 @pytest.mark.parametrize("name,dim", [("f16", 128), ("bf16", 64)])
-@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (16, 0), (100, 4), (100, 130), (5000, 4)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (16, 0), (100, 4), (100, 130), (5000, 4),
+                                          (2 ** 32 - 1, 2 ** 32 - 1)])
 def test_attention_few_rows_window(name, dim, window, sinks):
     b = P.Batch(FEW, 2, 4, dim, 16, name, window=window, sinks=sinks)
     b.call()
@@ -211,7 +212,8 @@ def test_attention_many_rows(heads, gq, page, heads_first, name, dim):
 
 
 @pytest.mark.parametrize("window,sinks,page", [(1, 0, 16), (64, 0, 48), (64, 1, 16), (129, 4, 16), (200, 130, 64),
-                                               (128, 257, 32), (4096, 4, 16)])
+                                               (128, 257, 32), (4096, 4, 16),
+                                               (2 ** 32 - 1, 0, 16), (100, 2 ** 32 - 1, 16)])
 @pytest.mark.parametrize("name,dim", [("bf16", 128), ("f16", 64)])
 def test_attention_many_rows_window(window, sinks, page, name, dim):
     b = P.Batch(MANY + [(900, 1), (2000, 30)], 1, 3, dim, page, name, window=window, sinks=sinks)
@@ -318,6 +320,41 @@ def test_attention_other_stream_and_replay():
     for x in both:
         x.check()
     assert P.device_error() == 0
+
+
+def test_attention_beside_q_in_one_array():
+    """q and out as parts of the same rows."""
+    b = P.Batch([(30, 40), (90, 1)], 2, 4, dim=64)
+    n = b.qh * 64
+    both = torch.full((b.rows + 3, 2 * n + 8), 5.0, dtype=torch.float16, device=G.dev())
+    both[:b.rows, :n] = P.dev(b.q.flatten(1))
+    b.qd, b.out = both[:, :n], both[:, n:2 * n]
+    b.call()
+    b.out = torch.cat([b.out, torch.full_like(b.out, 5.0)], 1)
+    b.check()
+
+
+@pytest.mark.parametrize("lens", [[(100, 1), (40, 1)], [(100, 50), (40, 1)]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_of_scores_that_are_no_numbers(lens, bad):
+    """A query, or a visible key, that is not finite: the rows whose scores are NaN or +inf for it have no softmax (a
+    score of -inf, where q is negative, only has no weight), the others are as they were."""
+    b = P.Batch(lens, 1, 4)
+    b.qd[0, 3] = bad  # row 0, head 0
+    page = int(b.table[1, 1])
+    b.cache.k[page, 2, 0, 7] = bad  # position 18 of request 1
+    b.q[0, 0] = 0  # the plain form's place for it
+    b.call()
+    got = b.out.float().cpu()
+    rows = b.rows - 1
+    assert not torch.isfinite(got[0, :128]).any()
+    for h in range(4):
+        none = bad != bad or b.q[rows, h, 7] > 0
+        assert torch.isfinite(got[rows, 128 * h:128 * h + 128]).any() != none
+    want, tol = P.attention_plain(b.q[:rows], b.k[0], b.v[0], torch.arange(100, 100 + rows), b.scale, 0, 0, "f16")
+    off = (got[:rows, :512].double().view(rows, 4, 128) - want).abs() <= tol
+    off[0, 0] = True
+    assert off.all()
 
 
 def test_attention_repeats_bit_for_bit():
