@@ -79,11 +79,17 @@ __device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {  /
 // The CTAs' bests go to CTA 0's shared memory by asynchronous stores (a cluster
 // barrier would first drain every store: 4000 clocks), so no workspace, no
 // atomics on global memory and no order of arrival is involved.
+// Rows need not start on 16 bytes: token t is numbered t + a, a the elements
+// between the last 16-byte boundary and the row's first, so that vectors of V
+// numbers are aligned (the first and the last may be partly outside the row).
+// Without Shift every row starts on 16 bytes and a is 0: the checks that Shift
+// needs cost 64 instead of 56 us for 128 rows of 152064 fp32 (single numbers, as
+// where logits and out lie differently to 16 bytes, 147 us).
 // Many rows: HBM traffic of the logits in and out; finishing the named tokens
 // after the stream, with loads of their own, cost a third of its time again, and
 // bulk copies into shared memory ahead of it were slower than the loads in
 // registers.  One row: latency.
-template <typename T, int V>
+template <typename T, int V, bool Shift>
 __global__ void __launch_bounds__(kLogitsThreads, 2)
     logits_process_kernel(LogitsProcess p, uint32_t slice, uint32_t chunk, unsigned int* err) {
     extern __shared__ uint32_t smem[];  // named bits, bits before each word's, list; counts, last bias entries
@@ -99,16 +105,19 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
     if (gridDim.x > 1u) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_trigger();
     pdl_wait();  // logits come from the preceding kernels
-    const uint32_t v_begin = min(blockIdx.x * slice, p.vocab), v_end = min(v_begin + slice, p.vocab);
-    const T* in = static_cast<const T*>(p.logits) + (uint64_t)row * p.stride;
-    T* out = static_cast<T*>(p.out) + (uint64_t)row * p.out_stride;
+    const T* first_in = static_cast<const T*>(p.logits) + (uint64_t)row * p.stride;
+    const uint32_t a = Shift ? (uint32_t)(reinterpret_cast<uintptr_t>(first_in) / sizeof(T)) % V : 0u;
+    const T* in = first_in - a;  // by numbers
+    T* out = static_cast<T*>(p.out) + (uint64_t)row * p.out_stride - a;
+    const uint32_t row_end = a + p.vocab;
+    const uint32_t v_begin = min(blockIdx.x * slice, row_end), v_end = min(v_begin + slice, row_end);
     constexpr uint32_t U = V > 1 ? 4 : 16;  // vectors, or single values, in flight per thread
     T x[U][V];
-    auto load = [&](uint32_t i0, uint32_t i1) {  // of the part's tokens [i0, i1)
+    auto load = [&](uint32_t i0, uint32_t i1) {  // of the numbers [i0, i1)
 #pragma unroll
         for (uint32_t j = 0; j < U; ++j) {
             const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
-            if (i + V <= i1) {
+            if (i >= a && i + V <= i1) {
                 if constexpr (V > 1)
                     *reinterpret_cast<uint4*>(x[j]) = __ldcs(reinterpret_cast<const uint4*>(in + i));
                 else
@@ -116,7 +125,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < V; ++k)
-                    if (i + k < i1) x[j][k] = in[i + k];
+                    if (i + k >= a && i + k < i1) x[j][k] = in[i + k];
             }
         }
     };
@@ -141,13 +150,15 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
     const uint32_t n_words = (chunk + 31u) / 32u;
     uint32_t* named = smem;
     uint32_t* before = named + n_words;
-    uint32_t* list = before + n_words + 1u;  // token - chunk's first, top bit: of the prompt
+    uint32_t* list = before + n_words + 1u;  // number - chunk's first, top bit: of the prompt
     uint32_t* count = list + kList;
     uint32_t* last = count + kNamed;  // only with biases
     const bool any = n_hist != 0u || b1 != b0;
     Best best;
     for (uint32_t c0 = v_begin; c0 < v_end; c0 += chunk) {
         const uint32_t n = min(chunk, v_end - c0);
+        // a token's place in the chunk; n or more when it is of another chunk, or no token at all
+        auto number = [&](int32_t id) { return (uint32_t)id < p.vocab ? (uint32_t)id + a - c0 : n; };
         uint32_t n_named = 0, n_listed = 0;
         if (any) {
 #pragma unroll 1
@@ -165,7 +176,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
 #pragma unroll
                 for (uint32_t k = 0; k < E; ++k) {
                     const uint32_t e = e0 + k * kLogitsThreads + tid;
-                    id[k] = e < n_hist ? (uint32_t)__ldg(hist + e) - c0 : n;  // >= n: none of the chunk
+                    id[k] = e < n_hist ? number(__ldg(hist + e)) : n;
                 }
 #pragma unroll
                 for (uint32_t k = 0; k < E; ++k) {
@@ -180,7 +191,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
             }
 #pragma unroll 1
             for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads)
-                if (const uint32_t i = (uint32_t)p.bias_ids[e] - c0; i < n) name(i);
+                if (const uint32_t i = number(p.bias_ids[e]); i < n) name(i);
             __syncthreads();
             n_listed = s_listed;
             const uint32_t per = (n_words + kLogitsThreads - 1u) / kLogitsThreads;
@@ -243,7 +254,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                 const uint32_t entries = listed ? n_listed : n_hist;
 #pragma unroll 1
                 for (uint32_t e = tid; e < entries; e += kLogitsThreads) {
-                    const uint32_t entry = listed ? list[e] : (uint32_t)__ldg(hist + e) - c0;
+                    const uint32_t entry = listed ? list[e] : number(__ldg(hist + e));
                     const bool prompt = listed ? (entry & kPromptSeen) != 0u : e < n_prompt;
                     const uint32_t i = listed ? entry & ~kPromptSeen : entry;
                     if (i < s0 || i >= s1) continue;
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                 }
 #pragma unroll 1
                 for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads)
-                    if (const uint32_t i = (uint32_t)p.bias_ids[e] - c0; i >= s0 && i < s1)
+                    if (const uint32_t i = number(p.bias_ids[e]); i >= s0 && i < s1)
                         atomicMax(&last[place(i)], e - b0 + 1u);
                 __syncthreads();
             }
@@ -266,8 +277,15 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                 for (uint32_t j = 0; j < U; ++j) {
                     const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
                     if (i >= s1) continue;
-                    // V consecutive tokens start on a multiple of V, so their bits lie in one word
-                    const uint32_t allowed = mask ? __ldg(mask + ((c0 + i) >> 5)) >> ((c0 + i) & 31u) : 0xffffffffu;
+                    uint32_t allowed = 0xffffffffu;
+                    if (mask) {  // the vector's bits may reach into the next word
+                        const uint32_t t = max(c0 + i, a) - a, sh = t & 31u;
+                        allowed = __ldg(mask + (t >> 5)) >> sh;
+                        if (Shift && sh + V > 32u && (t >> 5) < (p.vocab - 1u) / 32u)
+                            allowed |= __ldg(mask + (t >> 5) + 1u) << (32u - sh);
+                        allowed <<= max(c0 + i, a) - (c0 + i);
+                    }
+                    // V consecutive numbers start on a multiple of V, so their bits lie in one word
                     const uint32_t here = n_named ? (named[i >> 5] >> (i & 31u)) & ((1u << V) - 1u) : 0u;
                     if (here) {
                         uint32_t r = place(i);
@@ -282,13 +300,13 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                     }
 #pragma unroll
                     for (uint32_t k = 0; k < V; ++k) {
-                        if (i + k >= s1) continue;
+                        if (i + k >= s1 || c0 + i + k < a) continue;
                         if (!((allowed >> k) & 1u))
                             from_f32(-INFINITY, x[j][k]);
                         else if (const float v = to_f32(x[j][k]); v > best.v && v < INFINITY)
-                            best.v = v, best.at = c0 + i + k;  // tokens ascend, so the first of equals stays
+                            best.v = v, best.at = c0 + i + k - a;  // tokens ascend, so the first of equals stays
                     }
-                    if (i + V <= s1) {
+                    if (c0 + i >= a && i + V <= s1) {
                         if constexpr (V > 1)
                             __stcs(reinterpret_cast<uint4*>(out + c0 + i), *reinterpret_cast<const uint4*>(x[j]));
                         else
@@ -296,7 +314,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                     } else {
 #pragma unroll
                         for (uint32_t k = 0; k < V; ++k)
-                            if (i + k < s1) out[c0 + i + k] = x[j][k];
+                            if (i + k < s1 && c0 + i + k >= a) out[c0 + i + k] = x[j][k];
                     }
                 }
             }
@@ -331,7 +349,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool Shift>
 cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, cudaStream_t stream) {
     // CTAs per row: as many as give the least waves x (tokens of a CTA + what a CTA costs beside them)
     constexpr uint64_t kSlots = 2u * 148u, kCtaCost = 7500u;
@@ -341,13 +359,13 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
         const uint64_t t = ((uint64_t)p.n_rows * c + kSlots - 1u) / kSlots * (p.vocab / c + kCtaCost);
         if (t < least) least = t, ctas = c;
     }
-    const uint32_t slice = ((p.vocab + ctas - 1u) / ctas + 31u) / 32u * 32u;
+    const uint32_t slice = ((p.vocab + V - 1u + ctas - 1u) / ctas + 31u) / 32u * 32u;
     const uint32_t chunk = std::min(slice, kChunk);
     const bool counts = p.history && (p.repetition || p.frequency || p.presence);
     const uint32_t smem = counts || p.bias_start
                               ? (chunk + 31u) / 32u * 8u + 4u + 4u * kList + 4u * kNamed * (p.bias_start ? 2u : 1u)
                               : 0u;
-    cudaError_t e = allow_shared<logits_process_kernel<T, V>, true>(kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
+    cudaError_t e = allow_shared<logits_process_kernel<T, V, Shift>, true>(kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
     if (e != cudaSuccess) return e;
     LogitsProcess q = p;
     q.n_rows = rows;
@@ -380,20 +398,22 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 2;
     }
-    e = cudaLaunchKernelEx(&cfg, logits_process_kernel<T, V>, q, slice, chunk, dev_error_word());
+    e = cudaLaunchKernelEx(&cfg, logits_process_kernel<T, V, Shift>, q, slice, chunk, dev_error_word());
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_logits_type(const LogitsProcess& p, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    const uintptr_t all = reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out);
-    // 16-byte vectors when every row starts on 16 bytes
-    const bool vec = (all & 15u) == 0u && p.stride % V == 0u && p.out_stride % V == 0u;
+    // 16-byte vectors when the rows of logits and out lie the same way to 16 bytes
+    const uintptr_t in = reinterpret_cast<uintptr_t>(p.logits), out = reinterpret_cast<uintptr_t>(p.out);
+    const bool vec = (in - out) % 16u == 0u && (p.stride - p.out_stride) % V == 0u;
+    const bool aligned = vec && in % 16u == 0u && p.stride % V == 0u;
+    const auto launch = aligned ? launch_logits<T, V, false> : vec ? launch_logits<T, V, true> : launch_logits<T, 1, false>;
     constexpr uint32_t kMaxGridY = 65535u;
     for (uint32_t r = 0; r < p.n_rows; r += kMaxGridY) {
         const uint32_t rows = std::min(kMaxGridY, p.n_rows - r);
-        const cudaError_t e = vec ? launch_logits<T, V>(p, r, rows, stream) : launch_logits<T, 1>(p, r, rows, stream);
+        const cudaError_t e = launch(p, r, rows, stream);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

@@ -49,13 +49,15 @@ def plain(x, history, prompt, total, rep, freq, pres, biases, mask, name):
 
 
 def run(x, history=None, prompt=None, total=None, rep=None, freq=None, pres=None, biases=None, mask=None, name="f32",
-        pad=0, off=0, in_place=False, want_best=True):
+        pad=0, off=0, in_place=False, want_best=True, out_off=None):
     rows, vocab = x.shape
     t = torch.from_numpy(x).to(P.DT[name])
     buf = torch.full((rows, vocab + pad + off), 7.0, dtype=P.DT[name], device=G.dev())
     xd = buf[:, off:off + vocab]
     xd.copy_(t)
-    out = xd if in_place else torch.full((rows, vocab + pad + off), 7.0, dtype=P.DT[name], device=G.dev())[:, off:off + vocab]
+    o = off if out_off is None else out_off
+    obuf = torch.full((rows, vocab + pad + o), 7.0, dtype=P.DT[name], device=G.dev())
+    out = xd if in_place else obuf[:, o:o + vocab]
     up = lambda v, ty: None if v is None else torch.from_numpy(np.ascontiguousarray(v, dtype=ty)).to(G.dev())  # noqa: E731
     hd, pd, td = up(history, np.int32), up(prompt, np.int32), up(total, np.int32)
     rd, fd, sd = up(rep, np.float32), up(freq, np.float32), up(pres, np.float32)
@@ -76,8 +78,9 @@ def run(x, history=None, prompt=None, total=None, rep=None, freq=None, pres=None
     same = (got == want) | (got.isnan() & want.isnan())
     assert same.all(), (~same).nonzero()[:4]
     assert best.tolist() == (pick if want_best else [-7] * rows)
-    if pad and not in_place:
-        assert (buf[:, off + vocab:] == 7.0).all()
+    assert (buf[:, off + vocab:] == 7.0).all() and (buf[:, :off] == 7.0).all()
+    if not in_place:
+        assert (obuf[:, o + vocab:] == 7.0).all() and (obuf[:, :o] == 7.0).all()
     return best.tolist()
 
 
@@ -107,6 +110,17 @@ def test_strides_and_in_place(name, pad, off):
     x, h, p, t, (rep, freq, pres), b, m = inputs(6, 5003, 64, 3, words=160)
     run(x, h, p, t, rep, freq, pres, b, m, name, pad, off)
     run(x, h, p, t, rep, freq, pres, b, m, name, pad, off, in_place=True)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 31, 33, 1025, 70001])
+def test_rows_that_start_anywhere(name, vocab):
+    x, h, p, t, (rep, freq, pres), b, m = inputs(5, vocab, 40, vocab)
+    for off in range(1, 8):
+        run(x, h, p, t, rep, freq, pres, b, m, name, off % 3, off)
+        run(x, h, p, t, rep, freq, pres, b, m, name, 1, off, in_place=True)
+    run(x, h, p, t, rep, freq, pres, b, m, name, 1, 3, out_off=4)
+    run(x, h, p, t, rep, freq, pres, b, m, name, 0, 1, out_off=0)
 
 
 def test_each_constraint_alone():
