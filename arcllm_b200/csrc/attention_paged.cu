@@ -84,8 +84,8 @@ struct Cursor {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowWarps * 32, 1)
     attn_paged_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                           PageMap heads, Args a, uint32_t slot_rows, uint32_t stages, Record* __restrict__ recs, float* __restrict__ parts,
-                           unsigned int* err) {
+                           PageMap heads, Args a, uint32_t slot_rows, uint32_t stages,
+                           Record* __restrict__ recs, float* __restrict__ parts, unsigned int* err) {
     constexpr uint32_t GB = D / 64 * 1024u;  // 8 positions: [64-dim part][8][128 bytes]
     constexpr uint32_t TILE = kRowTile / 8u * GB, STAGE = 2u * TILE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
             // 8(j & 1) + 2t, + 1.
             const uint32_t p_last = cc.q.p0 + cc.q.n - 1u;
             const uint32_t p_from = a.window && cc.q.p0 >= a.window ? cc.q.p0 - a.window + 1u : 0u;
-            const bool edge = p_tile + kRowTile - 1u > p_last || (p_tile < p_from && p_tile + kRowTile > a.sinks) ;
+            const bool edge = p_tile + kRowTile - 1u > p_last || (p_tile < p_from && p_tile + kRowTile > a.sinks);
             uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
             if (edge) {
 #pragma unroll
@@ -555,7 +555,7 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: heads side by side in a token, or one after another");
     if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31))
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: a stride past 2^40 bytes");
-    if (rows_meet(p.q, p.q_stride, p.out, p.out_stride, p.max_rows, width, 2u))
+    if (rows_meet(p.q, 2u * p.q_stride, 2u * width, p.out, 2u * p.out_stride, 2u * width, p.max_rows))
         return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: out overlaps q");
     if (p.workspace_bytes < need) return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: workspace too small");
     Args a{};

@@ -14,17 +14,29 @@
 //   warp 11           TMA: the next item's queries, as soon as the last S of the
 //                     item before is there
 // Tensor memory (512 columns of 128 rows) decides the tile: with O in 2 x D of
-// them, S and P of both halves fit side by side for 80 positions at D = 128 (at
-// D = 64 more; 96 is what a thread's registers hold).  With tiles of 128 at D = 128 P had to lie over S, S of the next
-// tile had to wait for the product, and the chain weights - products - S - softmax
-// of one half set the pace (3400 clocks for 128 positions); now S of the next tile
-// is formed as soon as a softmax has S in its registers.
+// them, S and P of both halves fit side by side for 80 positions at D = 128, so S
+// of the next tile is formed as soon as a softmax has S in its registers.  With
+// tiles of 128 P had to lie over S, S of the next tile had to wait for the
+// product, and the chain weights - products - S - softmax of one half set the
+// pace (3400 clocks for 128 positions, against 2290 for 80).  At D = 64 a tile is
+// 96 positions, what a thread's registers hold, and there is room for two P of
+// each half: P then needs no wait for the product before (12 requests, 16 heads,
+// window 1024: 105.0 -> 101.3 us).  Two P at D = 128 would leave tiles of 64
+// (12000 rows: 470 -> 504 us).
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
 // last time (the sums carry the same factor, so the result is the same).
 // K and V tiles are built from boxes of positions that divide the page and the
 // tile, so tiles and pages need not match.
 // All waits are bounded: on a timeout the roles leave their loops, drain what
 // they started and the error word is set.
+// Measured: 12000 new rows of 2 requests, 28 / 4 heads of 128, contexts of 2048
+// before them (0.50 TFLOP): 470 to 500 us, as the clock varies with the power,
+// so 1.0 to 1.07 PFLOP/s, 0.60 to 0.65 of the measured matrix rate.  The bound is
+// the softmax's chain per tile: 2290 clocks, of which the exponentials (16 per
+// clock and SM) are 960 and both halves' products 1460 beside them; the rest is
+// issue and hand-over (a wait that is over costs 100 clocks, and the chain has
+// three).  Starting the halves half a tile apart changed nothing, nor did none or
+// half of the exponentials on the FMA units instead of a quarter.
 #include <algorithm>
 
 #include "arcllm_cuda_internal.h"
@@ -52,9 +64,12 @@ struct Layout {
     static constexpr uint32_t kOff = kRing + kStages * kBytes;  // unit offsets of the requests
     // columns of tensor memory of half s
     static __device__ __forceinline__ uint32_t s_col(uint32_t s) { return s * kTile; }
-    static __device__ __forceinline__ uint32_t p_col(uint32_t s) { return 2u * kTile + s * (kTile / 2u); }
+    static constexpr uint32_t kPs = D == 128 ? 1u : 2u;  // P of a half: one, or of even and of odd tiles
+    static __device__ __forceinline__ uint32_t p_col(uint32_t s, uint32_t n) {  // for the half's tile n
+        return 2u * kTile + (s * kPs + n % kPs) * (kTile / 2u);
+    }
     static __device__ __forceinline__ uint32_t o_col(uint32_t s) { return 512u - 2u * D + s * D; }
-    static_assert(3u * kTile <= 512u - 2u * D, "S and P of both halves beside O");
+    static_assert((2u + kPs) * kTile <= 512u - 2u * D, "S and P of both halves beside O");
 };
 
 // An item costs about this many tiles beside its own (queries in, first S, last
@@ -234,7 +249,7 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_paged_tiles_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                             const __grid_constant__ CUtensorMap qmap, PageMap heads, Args a,
-                            uint32_t box, uint32_t least, Record* __restrict__ recs, float* __restrict__ parts,
+                            uint32_t box, Record* __restrict__ recs, float* __restrict__ parts,
                             unsigned int* err) {
     using L = Layout<D>;
     constexpr uint32_t kTile = L::kTile;
@@ -242,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
     __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2],
-        p_empty[2], o_full[2], done;
+        p_empty[2][L::kPs], o_full[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
@@ -255,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&s_full[s], 1);
             mbar_init(&s_empty[s], 4);
             mbar_init(&p_full[s], 4);
-            mbar_init(&p_empty[s], 1);
+            for (uint32_t k = 0; k < L::kPs; ++k) mbar_init(&p_empty[s][k], 1);
             mbar_init(&o_full[s], 1);
         }
         mbar_init(&done, 2);
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bad = any_bad;
         return off[r + 1];
     });
-    const uint32_t per = max((total + gridDim.x - 1u) / gridDim.x, least);
+    const uint32_t per = max((total + gridDim.x - 1u) / gridDim.x, 1u);
     const uint32_t U0 = (uint32_t)min((unsigned long long)blockIdx.x * per, (unsigned long long)total);
     const uint32_t n_units = __shfl_sync(0xffffffffu, min(per, total - U0), 0);
     if (tid == 0) recs[blockIdx.x].valid = 0;
@@ -404,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------- MMA of half s ----------------
         constexpr uint32_t kQk = instr_desc<BF16>(kTile, false), kPv = instr_desc<BF16>(D, true);
         const uint32_t s = warp - 9u, leader = lane == 0, ring = smem_addr(smem + L::kRing);
-        const uint32_t ts = tmem + L::s_col(s), tp = tmem + L::p_col(s), to = tmem + L::o_col(s);
+        const uint32_t ts = tmem + L::s_col(s), to = tmem + L::o_col(s);
         const uint64_t qa = operand_desc(smem_addr(smem) + s * L::kQBytes, 16u, 1024u);
         // Tiles come as K, V, K, V ...; K of the next one is used before V of this one.
         struct At {
@@ -467,13 +482,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                 }
                 if (live) {
-                    if (!wait(&p_full[s], n_p++ & 1u)) break;
+                    if (!wait(&p_full[s], n_p & 1u)) break;
+                    const uint32_t tp = tmem + L::p_col(s, n_p);
                     tmem_fence_after();
                     const uint64_t vb = operand_desc(ring + at_v.stage * L::kBytes, 1024u, L::kGroup);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kTile / 16u; ++kk)
                         mma_tmem(to, tp + kk * 8u, vb + kk * (2u * L::kGroup >> 4), kPv, i != i0 || kk != 0u, leader);
-                    mma_commit(&p_empty[s], leader);
+                    mma_commit(&p_empty[s][n_p++ % L::kPs], leader);
                     if (i + 1u == i1) mma_commit(&o_full[s], leader);
                 }
                 mma_commit(&kv_empty[at_v.stage], leader);
@@ -515,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------- softmax of half s: thread t has packed row t ----------------
         const uint32_t s = warp >> 2, t = tid & 127u;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
-        const uint32_t ts = tmem + lanes + L::s_col(s), tp = tmem + lanes + L::p_col(s), to = tmem + lanes + L::o_col(s);
+        const uint32_t ts = tmem + lanes + L::s_col(s), to = tmem + lanes + L::o_col(s);
         uint32_t n_s = 0, n_o = 0;  // tiles, items so far
         const uint32_t t_row = t / a.gq;
         bool ok = true;
@@ -566,9 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // An infinite score has no softmax: NaN for the row, as for a NaN score.
                 float mn = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.scale_log2;
                 if (mn == INFINITY) mn = NAN;
-                bool waited = n_s == 0u;  // for the product before: P's columns, and O
+                bool waited = n_s == 0u;  // for the product before: O, and P's columns where the half has one P
                 auto product = [&]() {
-                    if (!waited) ok = role_wait(&p_empty[s], (n_s - 1u) & 1u, &abort_flag, err);
+                    const uint32_t n = n_s - 1u;
+                    if (!waited) ok = role_wait(&p_empty[s][n % L::kPs], n / L::kPs & 1u, &abort_flag, err);
                     waited = true;
                     tmem_fence_after();
                     return ok;
@@ -612,8 +629,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // the product takes weights of the cache's type: half a step of it each, as the output
                         pk[c / 2u] = pack16<BF16>(e.x, e.y);
                     }
-                    if (c0 == 0u && !product()) break;
-                    tmem_st(tp + c0 / 2u, pk);
+                    // Of two Ps this one's last product came before this S on the tensor core: it is over.
+                    if (L::kPs == 1u && c0 == 0u && !product()) break;
+                    tmem_st(tmem + lanes + L::p_col(s, n_s) + c0 / 2u, pk);
                 }
                 if (!ok) break;
                 const float2 sm = unpair(add2(sum[0], sum[1]));
@@ -712,7 +730,7 @@ int launch_tiles(const arcllm_cuda_paged_kv& kv, const Args& a, Record* recs, fl
     cudaError_t e = allow_shared<attn_paged_tiles_kernel<D, BF16>>((int)(1024u + L::kOff + 4u * (kMaxRequests + 1u)));
     if (e == cudaSuccess)
         e = launch_kernel(attn_paged_tiles_kernel<D, BF16>, dim3(kSms), dim3(kThreads), smem, stream, kmap, vmap,
-                          qmap, heads, a, box, 1u, recs, parts, dev_error_word());
+                          qmap, heads, a, box, recs, parts, dev_error_word());
     return e == cudaSuccess ? ARC_OK : set_cuda_error(e, "attention paged tiles launch");
 }
 

@@ -437,9 +437,13 @@ int rope_kv_paged(int act_type, const RopePaged& p, const arcllm_cuda_paged_kv& 
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: a row stride shorter than the row");
     const uint64_t as = act_type == ARC_GGML_F32 ? 4u : 2u;
     // in place (the same rows of the same type) or apart
-    if (p.q == p.q_out ? act_type != kv.type || p.q_stride != p.out_stride
-                       : rows_meet(p.q, p.q_stride * as, p.q_out, p.out_stride * 2u, p.rows, qn * std::max<uint64_t>(as, 2u), 1u))
+    auto meets_out = [&](const void* x, uint64_t stride, uint64_t width) {
+        return rows_meet(x, stride * as, width * as, p.q_out, p.out_stride * 2u, qn * 2u, p.rows);
+    };
+    if (p.q == p.q_out ? act_type != kv.type || p.q_stride != p.out_stride : meets_out(p.q, p.q_stride, qn))
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: q_out overlaps q without being the same rows");
+    if (meets_out(p.k, p.k_stride, kn) || meets_out(p.v, p.v_stride, kn))
+        return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: q_out overlaps k or v");
     // 16-byte vectors where every vector starts on 16 bytes and no unit is part rotated; else element by element
     const bool vec = p.rot_dim % 16u == 0u && kv.head_dim % 16u == 0u && aligned16(p.q) && aligned16(p.k) &&
                      aligned16(p.v) && aligned16(p.q_out) && aligned16(kv.k_pages) && aligned16(kv.v_pages) &&

@@ -1,5 +1,5 @@
 // Internal interface of the paged-cache serving kernels (paged_ops.cu,
-// logits_ops.cu, attention_paged.cu).
+// logits_ops.cu, attention_paged.cu, attention_paged_tiles.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -69,16 +69,15 @@ struct LogitsProcess {
 };
 int logits_process(int type, const LogitsProcess& p, cudaStream_t stream);
 
-// Whether two arrays of rows of `width` elements of `size` bytes share a byte.  Rows of one stride may lie side by
-// side in one array (parts of a fused projection); with different strides any overlap of the whole ranges counts.
-inline bool rows_meet(const void* a, uint64_t a_stride, const void* b, uint64_t b_stride, uint64_t rows,
-                      uint64_t width, uint64_t size) {
+// Whether two arrays of rows share a byte (strides and widths in bytes).  Rows of one stride may lie side by side
+// in one array (parts of a fused projection); with different strides any overlap of the whole ranges counts.
+inline bool rows_meet(const void* a, uint64_t a_stride, uint64_t a_width, const void* b, uint64_t b_stride,
+                      uint64_t b_width, uint64_t rows) {
     const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    const uint64_t na = ((rows - 1u) * a_stride + width) * size, nb = ((rows - 1u) * b_stride + width) * size;
-    if (x >= y + nb || y >= x + na) return false;
+    if (x >= y + (rows - 1u) * b_stride + b_width || y >= x + (rows - 1u) * a_stride + a_width) return false;
     if (a_stride != b_stride) return true;
-    const uint64_t off = (x > y ? x - y : y - x) % (a_stride * size);
-    return off < width * size || a_stride * size - off < width * size;
+    const uint64_t off = y >= x ? (y - x) % a_stride : a_stride - (x - y) % a_stride;  // of b's rows in a's
+    return off < a_width || off + b_width > a_stride;
 }
 
 // Checks of a cache descriptor that every user of it makes (null pointers, shape, type, the 32-bit slot range).

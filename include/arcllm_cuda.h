@@ -453,8 +453,9 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_freqs(int scaling, uint32_t rot_dim, double
  *   layout     pairs (2i, 2i+1) as arcllm_cuda_rope_kv_rows, or (i, i + rot_dim/2);
  *   freqs      rot_dim/2 doubles (device).
  * Angles are formed in 64 bits, so positions are not limited by a table.
- * q_out may be q itself (same type, same stride).  Slots must differ from one
- * another.  16-byte aligned rows and rot_dim, head_dim % 16 == 0 take the
+ * q_out may be q itself (same type, same stride), and overlaps none of q, k, v
+ * otherwise.  Slots must differ from one another (of rows with one slot, any one
+ * may be stored).  16-byte aligned rows and rot_dim, head_dim % 16 == 0 take the
  * vector form. */
 enum arcllm_rope_layout { ARC_ROPE_INTERLEAVED = 0, ARC_ROPE_HALVES = 1 };
 ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint64_t q_stride, const void *k,
@@ -486,7 +487,10 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  * after another (head_stride = page_size * token_stride).
  * A request whose lengths do not fit (kv_total < n, n > max_new, a table row
  * too short, rows past max_rows) is skipped and sets the bounds bit; a page
- * number outside [0, n_pages) sets it too and reads as zeros. */
+ * number outside [0, n_pages) sets it too and reads as zeros.  What lies at
+ * positions that no row of a request sees may be anything; an infinite or NaN
+ * value at a position that one of its rows sees may make others of its rows NaN
+ * (a weight of 0 times it). */
 ARCLLM_CUDA_API int arcllm_cuda_attention_paged_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                                                           uint64_t *out);
 ARCLLM_CUDA_API int arcllm_cuda_attention_paged(const void *q, uint64_t q_stride, const arcllm_cuda_paged_kv *kv,
@@ -506,7 +510,7 @@ ARCLLM_CUDA_API int arcllm_cuda_attention_paged(const void *q, uint64_t q_stride
  *   an entry in the row's biases:  l += value (of several for one token the
  *                                  last one counts);
  *   mask bit 0:                    l = -inf.
- *   history      [n_rows][history_stride] tokens; [0, prompt_len) is the prompt
+ *   history      [n_rows][history_stride < 2^29] tokens; [0, prompt_len) is the prompt
  *                (prompt_len null: none), [prompt_len, total_len) generated;
  *                values outside the vocabulary are passed over;
  *   repetition, frequency, presence  [n_rows], each nullable;
@@ -514,7 +518,9 @@ ARCLLM_CUDA_API int arcllm_cuda_attention_paged(const void *q, uint64_t q_stride
  *   mask         [n_rows][mask_stride] words, bit t % 32 of word t / 32 set:
  *                token t is allowed; null: all are;
  *   out          of the logits' type (F32, F16 or BF16), rounded to it; may be
- *                logits itself with the same stride;
+ *                logits itself with the same stride, and is apart from it
+ *                otherwise; rows that lie the same way to 16 bytes in both are
+ *                read and written 16 bytes at a time;
  *   best         [n_rows] lowest index of the largest finite value of out, -1
  *                when there is none; null: not wanted. */
 ARCLLM_CUDA_API int arcllm_cuda_logits_process(int type, const void *logits, uint64_t stride, uint32_t n_rows,

@@ -181,3 +181,33 @@ def test_matches_argmax_of_the_library():
         i, ok = C.c_uint32(), C.c_int()
         A.call("arcllm_cuda_argmax", G.ptr(xd[r]), 152064, G.ptr(scratch), C.byref(i), C.byref(ok), G.stream())
         assert i.value == best[r] and ok.value == 1
+
+
+def test_captured_and_on_two_streams():
+    rows, vocab, hist = 7, 70001, 500
+    x, h, p, t, (rep, freq, pres), b, m = inputs(rows, vocab, hist, 11)
+    want, pick = plain(x, h, p, t, rep, freq, pres, None, m, "f32")
+    hd, pd, td, rd, fd, sd = (G.to_dev(np.ascontiguousarray(v)) for v in (
+        h.astype(np.int32), np.asarray(p, np.int32), np.asarray(t, np.int32), np.asarray(rep, np.float32),
+        np.asarray(freq, np.float32), np.asarray(pres, np.float32)))
+    md = G.to_dev(m.view(np.int32))
+    sets = [(G.to_dev(x), torch.zeros((rows, vocab), device=G.dev()), torch.zeros(rows, dtype=torch.int32, device=G.dev()))
+            for _ in range(3)]
+
+    def go(stream, xd, out, best):
+        A.call("arcllm_cuda_logits_process", A.GGML_F32, G.ptr(xd), vocab, rows, vocab, G.ptr(hd), hist, G.ptr(pd),
+               G.ptr(td), G.ptr(rd), G.ptr(fd), G.ptr(sd), None, None, None, G.ptr(md), m.shape[1], G.ptr(out), vocab,
+               G.ptr(best), C.c_void_p(stream.cuda_stream))
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=streams[0]):
+        go(streams[0], *sets[2])
+    for _ in range(5):
+        for st, v in zip(streams, sets):
+            go(st, *v)
+        g.replay()
+    torch.cuda.synchronize()
+    for _, out, best in sets:
+        assert (out.cpu() == want).all() and best.tolist() == pick

@@ -73,6 +73,16 @@ def test_rope_refusals():
     assert status(f, changed(half, 20, 520)) == INVALID  # other rows
     assert status(f, changed(changed(good, 0, A.GGML_F16), 19, P((3 << 20) + 1000))) == INVALID  # half a row on
     assert status(f, changed(good, 19, P((3 << 20) + 2048))) == INVALID  # row 1 of q
+    for i in (1, 2):  # k, v: rows of 512 bytes, 3 of them
+        assert status(f, changed(good, 19, a[i])) == INVALID
+        assert status(f, changed(good, 19, P(((3 + i) << 20) + 1520))) == INVALID
+    # q, k, v in one projection's rows (4 + 1 + 1 heads of 128 halves), q in place: not refused, over k refused
+    fused = changed(changed(changed(changed(half, 2, 768), 4, 768), 6, 768), 20, 768)
+    fused = changed(changed(fused, 3, P((3 << 20) + 1024)), 5, P((3 << 20) + 1280))
+    assert status(f, fused) != INVALID
+    assert status(f, changed(fused, 19, P((3 << 20) + 16))) == INVALID
+    assert status(f, changed(fused, 3, P((3 << 20) + 1008))) == INVALID
+    assert status(f, changed(fused, 5, P((3 << 20) + 1536 + 1008))) == INVALID  # the next row's q
 
 
 def test_attention_refusals():

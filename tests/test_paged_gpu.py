@@ -145,6 +145,45 @@ def test_rope_in_place_and_far_positions(name):
     rope_case("f32", name, 8, 2, 128, 64, False, 16, True, False, 21, far=2 ** 31 - 1)
 
 
+def test_rope_of_one_projection_in_place_captured_and_on_two_streams():
+    """q, k, v as parts of the same rows, q rotated where it stands; every way of calling gives the same bits."""
+    rows, qh, heads, dim, name = 70, 6, 2, 128, "bf16"
+    qn, kn = qh * dim, heads * dim
+    x = P.normal((rows, qn + 2 * kn), 31, name)
+    pos = torch.arange(rows) * 1000
+    f, s = P.frequencies(dim)
+    fd, pd, sd = P.dev(f), P.i32(pos.tolist()), P.i32(range(rows))
+    want = P.rotate(x[:, :qn].double().view(rows, qh, dim), pos, f, s, True)
+
+    def go(stream, xd, cache):
+        A.call("arcllm_cuda_rope_kv_paged", P.GGML[name], G.ptr(xd), xd.stride(0), G.ptr(xd[:, qn:]), xd.stride(0),
+               G.ptr(xd[:, qn + kn:]), xd.stride(0), None, None, None, G.ptr(fd), dim, A.ROPE_HALVES, s, G.ptr(pd),
+               G.ptr(sd), rows, qh, cache.ref(), G.ptr(xd), xd.stride(0), C.c_void_p(stream.cuda_stream))
+
+    sets = [(P.dev(x), P.Cache(5, 16, heads, dim, name, i == 1)) for i in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=streams[0]):
+        go(streams[0], *sets[2])
+    assert (sets[2][0].cpu() == x).all()
+    for st, v in zip(streams, sets):
+        go(st, *v)
+    g.replay()
+    torch.cuda.synchronize()
+    first = sets[0][0].cpu()
+    # one product each and their sum in fp32, angles and their sines to 2^-22, then the type's half step
+    size = x[:, :qn].double().view(rows, qh, dim).abs()
+    tol = P.half_step(name) * want.abs() + (size + size.roll(dim // 2, -1)) * 2.0 ** -20
+    assert ((first[:, :qn].double().view(rows, qh, dim) - want).abs() <= tol).all()
+    assert (first[:, qn:] == x[:, qn:]).all()
+    for xd, cache in sets:
+        assert (xd.cpu() == first).all()
+        assert (cache.v.reshape(-1, heads, dim)[:rows].cpu().flatten(1) == x[:, qn + kn:]).all()
+        assert (cache.k.reshape(-1, heads, dim)[:rows] == sets[0][1].k.reshape(-1, heads, dim)[:rows]).all()
+    assert P.device_error() == 0
+
+
 def test_rope_slots_outside_the_cache_are_skipped():
     cache = P.Cache(2, 16, 1, 64, "f16", False, 5.0)
     x = torch.zeros((4, 64), dtype=torch.float16, device=G.dev())
@@ -319,6 +358,23 @@ def test_attention_other_stream_and_replay():
     torch.cuda.synchronize()
     for x in both:
         x.check()
+    assert P.device_error() == 0
+
+
+@pytest.mark.parametrize("lens", [[(5, 1)] * 4096, [(2, 17)] * 400 + [(0, 0)] * 3000 + [(40, 1)]])
+def test_attention_many_requests(lens):
+    b = P.Batch(lens, 1, 1, 64, 16, "f16")
+    b.call(max_new=2 ** 32 - 1)
+    b.check()
+    assert P.device_error() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,gq", [([(0, 17)], 1), ([(9, 1)], 20), ([(0, 6)], 3)])
+def test_attention_fewer_rows_than_a_tile_takes(dim, lens, gq):
+    b = P.Batch(lens, 1, gq, dim, 16, "bf16", spare_rows=0)
+    b.call()
+    b.check()
     assert P.device_error() == 0
 
 
