@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align_up<1024>(smem_raw, 0);
     uint32_t* off = reinterpret_cast<uint32_t*>(smem + L::kOff);
-    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], s_empty[2], p_full[2],
-        p_empty[2][L::kPs], o_full[2], done;
+    __shared__ uint64_t kv_full[L::kStages], kv_empty[L::kStages], q_full[2], q_empty[2], s_full[2], s_empty[2],
+        p_full[2][L::kPs], p_empty[2][L::kPs], o_full[2], done;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     __shared__ uint32_t start[4];
@@ -269,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&q_empty[s], 1);
             mbar_init(&s_full[s], 1);
             mbar_init(&s_empty[s], 4);
-            mbar_init(&p_full[s], 4);
-            for (uint32_t k = 0; k < L::kPs; ++k) mbar_init(&p_empty[s][k], 1);
+            for (uint32_t k = 0; k < L::kPs; ++k) mbar_init(&p_full[s][k], 4), mbar_init(&p_empty[s][k], 1);
             mbar_init(&o_full[s], 1);
         }
         mbar_init(&done, 2);
@@ -482,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                 }
                 if (live) {
-                    if (!wait(&p_full[s], n_p & 1u)) break;
+                    if (!wait(&p_full[s][n_p % L::kPs], n_p / L::kPs & 1u)) break;
                     const uint32_t tp = tmem + L::p_col(s, n_p);
                     tmem_fence_after();
                     const uint64_t vb = operand_desc(ring + at_v.stage * L::kBytes, 1024u, L::kGroup);
@@ -629,18 +628,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // the product takes weights of the cache's type: half a step of it each, as the output
                         pk[c / 2u] = pack16<BF16>(e.x, e.y);
                     }
-                    // Of two Ps this one's last product came before this S on the tensor core: it is over.
+                    // Of two Ps this one's last product came before this S on the tensor core: it is over.  A warp may
+                    // then be one tile ahead of another of its half, so each P has a barrier of its own, too.
                     if (L::kPs == 1u && c0 == 0u && !product()) break;
                     tmem_st(tmem + lanes + L::p_col(s, n_s) + c0 / 2u, pk);
                 }
                 if (!ok) break;
                 const float2 sm = unpair(add2(sum[0], sum[1]));
                 l += sm.x + sm.y;
-                ++n_s;
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[s]);
+                if (lane == 0) mbar_arrive(&p_full[s][n_s % L::kPs]);
+                ++n_s;
             }
             if (ok) ok = role_wait(&o_full[s], n_o & 1u, &abort_flag, err);
             if (!ok) break;

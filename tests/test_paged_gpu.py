@@ -422,6 +422,21 @@ def test_attention_repeats_bit_for_bit():
         assert (G.host(b.out.view(torch.int16)) == first).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1024, 4)])
+def test_attention_long_work_repeats_bit_for_bit(dim, window, sinks):
+    """Enough tiles per SM for its warps to drift apart."""
+    b = P.Batch([(2500, 700), (100, 900)], 8, 2, dim, 32, "bf16", window=window, sinks=sinks)
+    b.call()
+    b.check()
+    first = b.out.view(torch.int16).clone()
+    for _ in range(200):
+        b.out.fill_(5.0)
+        b.call()
+        assert torch.equal(b.out.view(torch.int16), first)
+    assert P.device_error() == 0
+
+
 # ---- all of them together ---------------------------------------------------
 def test_steps_of_a_batch():
     """Prompts, then tokens, through plan, rotary store, attention and the
