@@ -21,7 +21,7 @@
 // pace (3400 clocks for 128 positions, against 2290 for 80).  At D = 64 a tile is
 // 96 positions, what a thread's registers hold, and there is room for two P of
 // each half: P then needs no wait for the product before (12 requests, 16 heads,
-// window 1024: 105.0 -> 101.3 us).  Two P at D = 128 would leave tiles of 64
+// window 1024: 105.2 -> 103.2 us).  Two P at D = 128 would leave tiles of 64
 // (12000 rows: 470 -> 504 us).
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
 // last time (the sums carry the same factor, so the result is the same).

@@ -200,61 +200,60 @@ __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
 // A unit is 2V elements of one head as two V-wide vectors: the two sides of V
 // rotated pairs in the half layout, 2V neighbours otherwise; it is read and
 // written by one thread, so q may be rotated in place.  Units of a head: rotated
-// ones first.  An item is a unit for each thread of the CTA (part w % parts of row
-// w / parts); a CTA walks over items and reads the next one before it turns to
-// the current one, for which the angles are in shared memory after one barrier.
+// ones first.  A thread keeps its unit and walks over rows (a CTA has part
+// blockIdx % parts of them); the next row is read before it turns to the current
+// one, for which the angles are in shared memory after one barrier.
 // Angles pos * freq are formed and reduced to a fraction of a turn in 64 bits
 // (at 16384 an fp32 product is already 1e-3 off), then sin and cos in fp32.
-// Bounded by HBM traffic for many rows and by latency for few.
+// Bounded by HBM traffic for many rows and by latency for few: 8192 rows of 32 / 8
+// heads of 128, bf16, 43 us (4.7 TB/s; 64 us with a row per CTA and none read
+// ahead, 48 with the unit worked out anew for each row), fp32 51 us (5.9 TB/s); 48
+// rows 3.1 us.  Two or three rows ahead, 3 or 4 CTAs' worth of threads per SM, or
+// units of 32 elements were 0 to 40 % slower, and without the angles it takes the same.
 constexpr uint32_t kRopeThreads = 512;
 template <typename TA, typename TC, int V>
 __global__ void __launch_bounds__(kRopeThreads) rope_kv_paged_kernel(RopePaged p, arcllm_cuda_paged_kv kv,
-                                                                     uint32_t parts, uint32_t items,
-                                                                     unsigned int* err) {
+                                                                     uint32_t parts, unsigned int* err) {
     pdl_trigger();
     pdl_wait();  // q, k, v come from the preceding kernels
     extern __shared__ float2 rope_smem[];  // (cos, sin) * attn_scale of rot_dim / 2 pairs, twice
     const uint32_t d = kv.head_dim, half = p.rot_dim / 2u;
     const uint32_t per_head = d / (2u * V), rot_units = half / V, rot_heads = p.q_heads + kv.kv_heads;
-    const uint32_t units = (rot_heads + kv.kv_heads) * per_head;
+    const uint32_t u = blockIdx.x % parts * blockDim.x + threadIdx.x;
+    const bool live = u < (rot_heads + kv.kv_heads) * per_head;
+    const uint32_t head = u / per_head, at = u - head * per_head;  // head of q, k, v in a row; its unit
+    const bool is_q = head < p.q_heads, turned = at < rot_units && head < rot_heads;
+    const bool halves = p.half_layout && turned;
+    const uint32_t oa = halves ? at * V : 2u * at * V;  // places of the vectors in the head
+    const uint32_t ob = halves ? half + at * V : oa + V;
+    const uint32_t in_part = is_q ? head : head < rot_heads ? head - p.q_heads : head - rot_heads;
+    const TA* src = static_cast<const TA*>(is_q ? p.q : head < rot_heads ? p.k : p.v) + in_part * d;
+    const uint64_t src_stride = is_q ? p.q_stride : head < rot_heads ? p.k_stride : p.v_stride;
+    const float* bias = is_q ? p.bq : head < rot_heads ? p.bk : p.bv;
     struct Item {
-        uint32_t row, head, at, oa, ob;  // head of q, k, v in a row; its unit; places of the vectors in the head
         int32_t slot, pos;
-        bool live, turned;
         Raw<TA, V> a, b;
     };
-    auto fetch = [&](uint32_t w, Item& x) {
-        x.row = w / parts;
-        const uint32_t u = (w - x.row * parts) * blockDim.x + threadIdx.x;
-        x.live = u < units;
-        x.slot = __ldg(p.slots + x.row);
-        x.pos = __ldg(p.positions + x.row);
-        x.head = u / per_head;
-        x.at = u - x.head * per_head;
-        x.turned = x.at < rot_units && x.head < rot_heads;
-        const bool halves = p.half_layout && x.turned;
-        x.oa = halves ? x.at * V : 2u * x.at * V;
-        x.ob = halves ? half + x.at * V : x.oa + V;
-        if (!x.live) return;
-        const TA* src = x.head < p.q_heads ? static_cast<const TA*>(p.q) + (uint64_t)x.row * p.q_stride + x.head * d
-                        : x.head < rot_heads
-                            ? static_cast<const TA*>(p.k) + (uint64_t)x.row * p.k_stride + (x.head - p.q_heads) * d
-                            : static_cast<const TA*>(p.v) + (uint64_t)x.row * p.v_stride + (x.head - rot_heads) * d;
-        x.a.load(src + x.oa);
-        x.b.load(src + x.ob);
+    auto fetch = [&](uint32_t row, Item& x) {
+        x.slot = __ldg(p.slots + row);
+        x.pos = __ldg(p.positions + row);
+        if (!live) return;
+        x.a.load(src + row * src_stride + oa);
+        x.b.load(src + row * src_stride + ob);
     };
+    const uint32_t step = gridDim.x / parts;
     Item next;
-    fetch(blockIdx.x, next);
+    fetch(blockIdx.x / parts, next);
     float2* angles = rope_smem;
-    for (uint32_t w = blockIdx.x; w < items; w += gridDim.x) {
+    for (uint32_t row = blockIdx.x / parts; row < p.rows; row += step) {
         const Item x = next;
-        if (items - w > gridDim.x) fetch(w + gridDim.x, next);
+        if (p.rows - row > step) fetch(row + step, next);
         if (x.slot < 0) continue;  // a row without a request (the same for all threads)
         if ((uint32_t)x.slot >= kv.n_pages * kv.page_size || x.pos < 0) {
             if (threadIdx.x == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
             continue;
         }
-        angles = angles == rope_smem ? rope_smem + half : rope_smem;  // others may still read the last item's
+        angles = angles == rope_smem ? rope_smem + half : rope_smem;  // others may still read the last row's
         for (uint32_t i = threadIdx.x; i < half; i += blockDim.x) {
             const double turns = (double)x.pos * p.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
             float s, c;
@@ -262,21 +261,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kv_paged_kernel(RopePaged p
             angles[i] = make_float2(c * p.attn_scale, s * p.attn_scale);
         }
         __syncthreads();
-        if (!x.live) continue;
-        const float* bias = x.head < p.q_heads ? p.bq : x.head < rot_heads ? p.bk : p.bv;
-        const uint32_t in_part = x.head < p.q_heads ? x.head : x.head < rot_heads ? x.head - p.q_heads : x.head - rot_heads;
+        if (!live) continue;
         float za[V], zb[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) za[i] = x.a[i], zb[i] = x.b[i];
         if (bias) {
             Raw<float, V> ba, bb;
-            ba.load(bias + in_part * d + x.oa);
-            bb.load(bias + in_part * d + x.ob);
+            ba.load(bias + in_part * d + oa);
+            bb.load(bias + in_part * d + ob);
 #pragma unroll
             for (int i = 0; i < V; ++i) za[i] += ba[i], zb[i] += bb[i];
         }
-        if (x.turned) {
-            const float2* cs = angles + x.at * V;
+        if (turned) {
+            const float2* cs = angles + at * V;
             if (p.half_layout) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -299,15 +296,15 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kv_paged_kernel(RopePaged p
             }
         }
         TC* dst;
-        if (x.head < p.q_heads) {
-            dst = static_cast<TC*>(p.q_out) + (uint64_t)x.row * p.out_stride + x.head * d;
+        if (is_q) {
+            dst = static_cast<TC*>(p.q_out) + (uint64_t)row * p.out_stride + head * d;
         } else {
             const uint32_t page = (uint32_t)x.slot / kv.page_size, token = (uint32_t)x.slot - page * kv.page_size;
-            dst = static_cast<TC*>(x.head < rot_heads ? kv.k_pages : kv.v_pages) + (uint64_t)page * kv.page_stride +
+            dst = static_cast<TC*>(head < rot_heads ? kv.k_pages : kv.v_pages) + (uint64_t)page * kv.page_stride +
                   (uint64_t)token * kv.token_stride + (uint64_t)in_part * kv.head_stride;
         }
-        store_vec<V>(dst + x.oa, za);
-        store_vec<V>(dst + x.ob, zb);
+        store_vec<V>(dst + oa, za);
+        store_vec<V>(dst + ob, zb);
     }
 }
 
@@ -317,13 +314,12 @@ cudaError_t launch_rope(const RopePaged& p, const arcllm_cuda_paged_kv& kv, bool
     const uint32_t threads = std::min(kRopeThreads, (units + 31u) / 32u * 32u);
     const uint32_t parts = (units + threads - 1u) / threads;
     const uint64_t items = (uint64_t)p.rows * parts;
-    if (items > 0x7fffffffull) return cudaErrorInvalidValue;
     const size_t smem = (size_t)p.rot_dim * sizeof(float2);
     auto go = [&](auto kernel) {
-        // as many CTAs as fit the card, each with its share of the items
-        const uint32_t fit = 148u * std::max(1u, 1024u / threads);
+        // as many CTAs as fit the card, in whole sets of parts, each with its share of the rows
+        const uint32_t fit = std::max(148u * std::max(1u, 1024u / threads) / parts, 1u) * parts;
         return launch_kernel(kernel, dim3((uint32_t)std::min<uint64_t>(items, fit)), dim3(threads), smem, stream, p, kv,
-                             parts, (uint32_t)items, dev_error_word());
+                             parts, dev_error_word());
     };
     return vec ? go(rope_kv_paged_kernel<TA, TC, 8>) : go(rope_kv_paged_kernel<TA, TC, 1>);
 }
