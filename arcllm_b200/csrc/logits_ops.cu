@@ -28,6 +28,16 @@ __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
+// a value of the type in a word of shared memory
+__device__ __forceinline__ uint32_t to_bits(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint32_t to_bits(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint32_t to_bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ void from_bits(uint32_t w, float& o) { o = __uint_as_float(w); }
+__device__ __forceinline__ void from_bits(uint32_t w, __half& o) { o = __ushort_as_half((unsigned short)w); }
+__device__ __forceinline__ void from_bits(uint32_t w, __nv_bfloat16& o) {
+    o = __ushort_as_bfloat16((unsigned short)w);
+}
+
 // larger float -> larger unsigned, -0 as +0 (the order of arcllm_cuda_argmax)
 __device__ __forceinline__ uint32_t ordered(float f) {
     uint32_t u = __float_as_uint(f);
@@ -152,7 +162,8 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
     uint32_t* before = named + n_words;
     uint32_t* list = before + n_words + 1u;  // number - chunk's first, top bit: of the prompt
     uint32_t* count = list + kList;
-    uint32_t* last = count + kNamed;  // only with biases
+    uint32_t* which = count + kNamed;  // numbers (less the chunk's first) of the named tokens, by place
+    uint32_t* last = which + kNamed;   // only with biases
     const bool any = n_hist != 0u || b1 != b0;
     Best best;
     for (uint32_t c0 = v_begin; c0 < v_end; c0 += chunk) {
@@ -222,7 +233,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
         if (any && tid == 0) before[n_words] = n_named;
         // As many words of bits at a time as name kNamed tokens at most (nearly always all of them).
         for (uint32_t w0 = 0; w0 * 32u < n;) {
-            uint32_t w1 = n_words, first = 0;
+            uint32_t w1 = n_words, first = 0, held = 0;
             if (n_named) {
                 __syncthreads();  // `before` is complete; the words of the round before are done with
                 first = before[w0];
@@ -237,10 +248,15 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                     }
                     w1 = lo;
                 }
-                const uint32_t held = before[w1] - first;
+                held = before[w1] - first;
                 for (uint32_t i = tid; i < held; i += kLogitsThreads) {
                     count[i] = 0u;
                     if (p.bias_start) last[i] = 0u;
+                }
+#pragma unroll 1
+                for (uint32_t w = w0 + tid; w < w1; w += kLogitsThreads) {
+                    uint32_t bits = named[w], r = before[w] - first;
+                    for (; bits; bits &= bits - 1u) which[r++] = w * 32u + (uint32_t)__ffs(bits) - 1u;
                 }
                 __syncthreads();
             }
@@ -250,6 +266,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
             };
             const uint32_t s0 = w0 * 32u, s1 = min(w1 * 32u, n);
             if (n_named) {
+                constexpr uint32_t G = kNamed / kLogitsThreads;
+                T own[G];  // logits of the named tokens, on their way while these are counted
+#pragma unroll
+                for (uint32_t k = 0; k < G; ++k)
+                    if (const uint32_t r = tid + k * kLogitsThreads; r < held) own[k] = in[c0 + which[r]];
                 const bool listed = n_listed <= kList;  // otherwise the history is read again
                 const uint32_t entries = listed ? n_listed : n_hist;
 #pragma unroll 1
@@ -268,6 +289,15 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                 for (uint32_t e = b0 + tid; e < b1; e += kLogitsThreads)
                     if (const uint32_t i = number(p.bias_ids[e]); i >= s0 && i < s1)
                         atomicMax(&last[place(i)], e - b0 + 1u);
+                __syncthreads();
+#pragma unroll
+                for (uint32_t k = 0; k < G; ++k)
+                    if (const uint32_t r = tid + k * kLogitsThreads; r < held) {
+                        float v = constrained(to_f32(own[k]), count[r], rp);
+                        if (p.bias_start && last[r]) v = __fadd_rn(v, p.bias_values[b0 + last[r] - 1u]);
+                        from_f32(v, own[k]);
+                        count[r] = to_bits(own[k]);  // what the stream puts in the token's place
+                    }
                 __syncthreads();
             }
 #pragma unroll 1
@@ -292,29 +322,36 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
 #pragma unroll
                         for (uint32_t k = 0; k < V; ++k) {
                             if (!((here >> k) & 1u)) continue;
-                            float v = constrained(to_f32(x[j][k]), count[r], rp);
-                            if (p.bias_start && last[r]) v = __fadd_rn(v, p.bias_values[b0 + last[r] - 1u]);
-                            from_f32(v, x[j][k]);
-                            ++r;
+                            from_bits(count[r++], x[j][k]);
                         }
                     }
+                    const uint32_t at = c0 + i;
+                    if (at >= a && i + V <= s1) {
+                        float top = -INFINITY;
 #pragma unroll
-                    for (uint32_t k = 0; k < V; ++k) {
-                        if (i + k >= s1 || c0 + i + k < a) continue;
-                        if (!((allowed >> k) & 1u))
-                            from_f32(-INFINITY, x[j][k]);
-                        else if (const float v = to_f32(x[j][k]); v > best.v && v < INFINITY)
-                            best.v = v, best.at = c0 + i + k - a;  // tokens ascend, so the first of equals stays
-                    }
-                    if (c0 + i >= a && i + V <= s1) {
+                        for (uint32_t k = 0; k < V; ++k) {
+                            if (!((allowed >> k) & 1u)) from_f32(-INFINITY, x[j][k]);
+                            top = fmaxf(top, to_f32(x[j][k]));  // passes over NaN
+                        }
+                        if (top == INFINITY) {  // not a choice: the largest of the others
+                            top = -INFINITY;
+#pragma unroll
+                            for (uint32_t k = 0; k < V; ++k)
+                                if (const float v = to_f32(x[j][k]); v < INFINITY) top = fmaxf(top, v);
+                        }
+                        if (top > best.v) best.v = top, best.at = at;  // numbers ascend, so the first of equals stays
                         if constexpr (V > 1)
-                            __stcs(reinterpret_cast<uint4*>(out + c0 + i), *reinterpret_cast<const uint4*>(x[j]));
+                            __stcs(reinterpret_cast<uint4*>(out + at), *reinterpret_cast<const uint4*>(x[j]));
                         else
-                            out[c0 + i] = x[j][0];
-                    } else {
+                            out[at] = x[j][0];
+                    } else {  // partly outside the row
 #pragma unroll
-                        for (uint32_t k = 0; k < V; ++k)
-                            if (i + k < s1 && c0 + i + k >= a) out[c0 + i + k] = x[j][k];
+                        for (uint32_t k = 0; k < V; ++k) {
+                            if (i + k >= s1 || at + k < a) continue;
+                            if (!((allowed >> k) & 1u)) from_f32(-INFINITY, x[j][k]);
+                            if (const float v = to_f32(x[j][k]); v > best.v && v < INFINITY) best.v = v, best.at = at;
+                            out[at + k] = x[j][k];
+                        }
                     }
                 }
             }
@@ -323,6 +360,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
         if (c0 + chunk < v_end) __syncthreads();  // bits and list are set anew
     }
     if (p.best) {
+        if (best.at != 0xffffffffu) {  // the first of its vector that has the value (the thread wrote it itself)
+            uint32_t t = max(best.at, a);
+            while (to_f32(out[t]) != best.v) ++t;
+            best.at = t - a;
+        }
         unsigned long long key = best.at == 0xffffffffu
                                      ? 0ull
                                      : ((unsigned long long)ordered(best.v) << 32) | (unsigned long long)(~best.at);
@@ -363,9 +405,9 @@ cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, 
     const uint32_t chunk = std::min(slice, kChunk);
     const bool counts = p.history && (p.repetition || p.frequency || p.presence);
     const uint32_t smem = counts || p.bias_start
-                              ? (chunk + 31u) / 32u * 8u + 4u + 4u * kList + 4u * kNamed * (p.bias_start ? 2u : 1u)
+                              ? (chunk + 31u) / 32u * 8u + 4u + 4u * kList + 4u * kNamed * (p.bias_start ? 3u : 2u)
                               : 0u;
-    cudaError_t e = allow_shared<logits_process_kernel<T, V, Shift>, true>(kChunk / 4 + 4 + 4 * kList + 8 * kNamed);
+    cudaError_t e = allow_shared<logits_process_kernel<T, V, Shift>, true>(kChunk / 4 + 4 + 4 * kList + 12 * kNamed);
     if (e != cudaSuccess) return e;
     LogitsProcess q = p;
     q.n_rows = rows;
