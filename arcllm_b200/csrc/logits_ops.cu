@@ -92,9 +92,9 @@ __device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {  /
 // Rows need not start on 16 bytes: token t is numbered t + a, a the elements
 // between the last 16-byte boundary and the row's first, so that vectors of V
 // numbers are aligned (the first and the last may be partly outside the row).
-// Without Shift every row starts on 16 bytes and a is 0: the checks that Shift
-// needs cost 64 instead of 56 us for 128 rows of 152064 fp32 (single numbers, as
-// where logits and out lie differently to 16 bytes, 147 us).
+// Without Shift every row starts on 16 bytes and a is 0: what Shift needs costs 44
+// instead of 41 us for 128 rows of 152064 fp32 (single numbers, as where logits and
+// out lie differently to 16 bytes, SINGLE us).
 // Many rows: HBM traffic of the logits in and out; finishing the named tokens
 // after the stream, with loads of their own, cost a third of its time again, and
 // bulk copies into shared memory ahead of it were slower than the loads in
@@ -303,18 +303,22 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
 #pragma unroll 1
             for (uint32_t i0 = s0; i0 < s1; i0 += kLogitsThreads * V * U) {
                 if (c0 + i0 != v_begin) load(c0 + i0, c0 + s1);
+                uint32_t allow[U];  // bit k: token k of the vector
+#pragma unroll
+                for (uint32_t j = 0; j < U; ++j) {
+                    const uint32_t at = c0 + i0 + (j * kLogitsThreads + tid) * V;
+                    allow[j] = 0xffffffffu;
+                    if (!mask || at >= c0 + s1) continue;
+                    const uint32_t t = max(at, a) - a, sh = t & 31u;
+                    allow[j] = __ldg(mask + (t >> 5)) >> sh;
+                    if (Shift && sh + V > 32u && (t >> 5) < (p.vocab - 1u) / 32u)  // reaches into the next word
+                        allow[j] |= __ldg(mask + (t >> 5) + 1u) << (32u - sh);
+                    allow[j] <<= max(at, a) - at;
+                }
 #pragma unroll
                 for (uint32_t j = 0; j < U; ++j) {
                     const uint32_t i = i0 + (j * kLogitsThreads + tid) * V;
                     if (i >= s1) continue;
-                    uint32_t allowed = 0xffffffffu;
-                    if (mask) {  // the vector's bits may reach into the next word
-                        const uint32_t t = max(c0 + i, a) - a, sh = t & 31u;
-                        allowed = __ldg(mask + (t >> 5)) >> sh;
-                        if (Shift && sh + V > 32u && (t >> 5) < (p.vocab - 1u) / 32u)
-                            allowed |= __ldg(mask + (t >> 5) + 1u) << (32u - sh);
-                        allowed <<= max(c0 + i, a) - (c0 + i);
-                    }
                     // V consecutive numbers start on a multiple of V, so their bits lie in one word
                     const uint32_t here = n_named ? (named[i >> 5] >> (i & 31u)) & ((1u << V) - 1u) : 0u;
                     if (here) {
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
                             from_bits(count[r++], x[j][k]);
                         }
                     }
-                    const uint32_t at = c0 + i;
+                    const uint32_t at = c0 + i, allowed = allow[j];
                     if (at >= a && i + V <= s1) {
                         float top = -INFINITY;
 #pragma unroll
