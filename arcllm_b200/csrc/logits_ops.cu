@@ -84,25 +84,30 @@ __device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {  /
 // place of its words (generated count, top bit: in the prompt; with biases 1 +
 // the index of its last entry), so shared memory holds words for the named tokens
 // only and a CTA's part can be long.  The history is read once, its entries of
-// the part kept in a list.  Then one stream over the logits reads, constrains,
-// masks and writes them and keeps the best finite value with the lowest index.
-// The CTAs' bests go to CTA 0's shared memory by asynchronous stores (a cluster
-// barrier would first drain every store: 4000 clocks), so no workspace, no
-// atomics on global memory and no order of arrival is involved.
+// the part kept in a list.  The named tokens' new values are worked out by place,
+// a thread for each, from logits gathered while they are counted.  Then one stream
+// over the logits reads, puts these values in, masks and writes, and keeps the
+// first vector with the largest finite value.  The CTAs' bests go to CTA 0's
+// shared memory by asynchronous stores (a cluster barrier would first drain every
+// store: 4000 clocks), so no workspace, no atomics on global memory and no order
+// of arrival is involved.
 // Rows need not start on 16 bytes: token t is numbered t + a, a the elements
 // between the last 16-byte boundary and the row's first, so that vectors of V
 // numbers are aligned (the first and the last may be partly outside the row).
 // Without Shift every row starts on 16 bytes and a is 0: what Shift needs costs 44
 // instead of 41 us for 128 rows of 152064 fp32 (single numbers, as where logits and
-// out lie differently to 16 bytes, SINGLE us).
-// Many rows: HBM traffic of the logits in and out; finishing the named tokens
-// after the stream, with loads of their own, cost a third of its time again, and
-// bulk copies into shared memory ahead of it were slower than the loads in
-// registers.  One row: latency.
+// out lie differently to 16 bytes, 110 us).
+// 128 rows of 152064 fp32 with histories of 4096, biases and masks: 41 us, 3.9
+// TB/s, of which counting is about 8 us with little traffic; without constraints
+// 31 us, 5.0 TB/s.  A row by itself: 7.8 us, latency.  Forming the named tokens in
+// the stream took 56 us (a warp nearly always has one, and then all of it waits for
+// the division), a choice token by token 47, mask words loaded where they are used
+// 43; bulk copies into shared memory ahead of the stream, or each register loaded
+// again as soon as its vector is written, were slower than this.
 template <typename T, int V, bool Shift>
 __global__ void __launch_bounds__(kLogitsThreads, 2)
     logits_process_kernel(LogitsProcess p, uint32_t slice, uint32_t chunk, unsigned int* err) {
-    extern __shared__ uint32_t smem[];  // named bits, bits before each word's, list; counts, last bias entries
+    extern __shared__ uint32_t smem[];  // named bits, bits before each word's, list; counts, numbers, last bias entries
     __shared__ unsigned long long s_best[kLogitsThreads / 32], s_keys[16];
     __shared__ uint64_t keys_in;
     __shared__ uint32_t s_sum[kLogitsThreads / 32], s_listed;
@@ -397,7 +402,9 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
 
 template <typename T, int V, bool Shift>
 cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, cudaStream_t stream) {
-    // CTAs per row: as many as give the least waves x (tokens of a CTA + what a CTA costs beside them)
+    // CTAs per row: as many as give the least waves x (tokens of a CTA + what a CTA costs beside them).  Measured for
+    // 152064 tokens with all constraints: 128 rows 73 / 48 / 53 / 69 us with 1 / 2 / 4 / 8, 64 rows 66 / 36 / 28 / 36, 20
+    // rows 62 / 34 / 23 / 20.
     constexpr uint64_t kSlots = 2u * 148u, kCtaCost = 7500u;
     uint32_t ctas = 1;
     uint64_t least = ~0ull;
