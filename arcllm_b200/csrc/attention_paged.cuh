@@ -15,7 +15,10 @@ namespace paged {
 
 constexpr uint32_t kSms = 148;          // one CTA per SM in both attention kernels
 constexpr uint32_t kTileRows = 256;     // packed rows of an item of the tile kernel
-constexpr uint32_t kRowMax = 16;        // requests with at most so many packed rows go to the rows kernel
+// Requests with at most so many packed rows go to the rows kernel, whose matrix operand has 16.  32 requests over
+// 4096 positions of 8 heads: 16 rows there 97 us (1 row 93), 17 rows in the tile kernel 119 us (32 rows 134); 64 over
+// 512: 40 and 53 us; 4 over 4096: 24 and 25 us.
+constexpr uint32_t kRowMax = 16;
 constexpr uint32_t kMaxRequests = 4096; // unit offsets of the requests in shared memory
 
 struct Args {
