@@ -183,6 +183,28 @@ def test_matches_argmax_of_the_library():
         assert i.value == best[r] and ok.value == 1
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,hist", [(200, 30000, 20000), (1, 70001, 40000), (3, 9000, 9000)])
+def test_histories_that_name_most_of_the_vocabulary(name, rows, vocab, hist):
+    """More named tokens, and more history entries, than a CTA holds at a time."""
+    x, h, p, t, (rep, freq, pres), b, m = inputs(rows, vocab, hist, 17)
+    r = np.random.default_rng(5)
+    for i in range(min(rows, 3)):
+        h[i] = r.permutation(vocab)[:hist]
+    t[:3] = hist
+    for i in range(3, rows):  # the others are short, for the plain form's sake
+        t[i] = min(t[i], 30)
+    run(x, h, p, t, rep, freq, pres, b, m, name)
+    run(x, h, p, t, rep, freq, pres, b, m, name, 1, 3, in_place=True)
+
+
+def test_rows_of_more_than_one_chunk():
+    x, h, p, t, (rep, freq, pres), b, m = inputs(296, 140003, 50, 23)
+    h[:, ::3] = 131000 + h[:, ::3] % 9003
+    run(x, h, p, t, rep, freq, pres, b, m, "f32")
+    run(x, h, p, t, rep, freq, pres, b, m, "f16", 0, 1)
+
+
 def test_captured_and_on_two_streams():
     rows, vocab, hist = 7, 70001, 500
     x, h, p, t, (rep, freq, pres), b, m = inputs(rows, vocab, hist, 11)
