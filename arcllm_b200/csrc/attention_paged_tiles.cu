@@ -33,10 +33,10 @@
 // before them (0.50 TFLOP): 470 to 500 us, as the clock varies with the power,
 // so 1.0 to 1.07 PFLOP/s, 0.60 to 0.65 of the measured matrix rate.  The bound is
 // the softmax's chain per tile: 2290 clocks, of which the exponentials (16 per
-// clock and SM) are 960 and both halves' products 1460 beside them; the rest is
+// clock and SM) are 1280 and both halves' products 1460 beside them; the rest is
 // issue and hand-over (a wait that is over costs 100 clocks, and the chain has
-// three).  Starting the halves half a tile apart changed nothing, nor did none or
-// half of the exponentials on the FMA units instead of a quarter.
+// three).  Starting the halves half a tile apart changed nothing, nor did a quarter
+// of the exponentials as polynomials on the FMA units (0.4 %; half of them 3 % slower).
 #include <algorithm>
 
 #include "arcllm_cuda_internal.h"
@@ -215,34 +215,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-// 2^y of a pair without the exponential unit (16 results per clock and SM, the
-// bound of this kernel's softmax): y = n + f with n the nearest integer (adding
-// 1.5 2^23 leaves it in the low mantissa bits), |f| <= 1/2, a polynomial for 2^f
-// (least relative error over +-1/2: degree 3 7.5e-5 = 2^-13.7 for bf16 weights,
-// degree 4 2.6e-6 = 2^-18.5 for fp16 ones) and n added to the exponent.  y below
-// -126 counts as -126.
-template <bool BF16>
-__device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
-    const float2 y = unpair(y2);
-    y2 = pair(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
-    const uint64_t t = add2(y2, pair(12582912.f, 12582912.f));
-    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), y2);
-    uint64_t p;
-    if constexpr (BF16) {
-        p = fma2(f, pair(0.0551716527f, 0.0551716527f), pair(0.242611121f, 0.242611121f));
-        p = fma2(p, f, pair(0.693260988f, 0.693260988f));
-        p = fma2(p, f, pair(0.999928074f, 0.999928074f));
-    } else {
-        p = fma2(f, pair(0.00957010002f, 0.00957010002f), pair(0.0559178602f, 0.0559178602f));
-        p = fma2(p, f, pair(0.240247449f, 0.240247449f));
-        p = fma2(p, f, pair(0.693121815f, 0.693121815f));
-        p = fma2(p, f, pair(0.999999261f, 0.999999261f));
-    }
-    const float2 q = unpair(p), n = unpair(t);
-    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
 }
 
 template <int D, bool BF16>
@@ -616,14 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t pk[kAtOnce / 2u];
 #pragma unroll
                     for (uint32_t c = 0; c < kAtOnce; c += 2u) {
-                        const uint64_t y2 = fma2(pair(x[c0 + c], x[c0 + c + 1u]), c2, r2);
-                        float2 e;
-                        if (c % 8u == 6u) {
-                            e = exp2_poly<BF16>(y2);
-                        } else {
-                            const float2 y = unpair(y2);
-                            e = make_float2(ex2(y.x), ex2(y.y));
-                        }
+                        const float2 y = unpair(fma2(pair(x[c0 + c], x[c0 + c + 1u]), c2, r2));
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
                         sum[(c >> 1) & 1u] = add2(sum[(c >> 1) & 1u], pair(e.x, e.y));
                         // the product takes weights of the cache's type: half a step of it each, as the output
                         pk[c / 2u] = pack16<BF16>(e.x, e.y);

@@ -132,9 +132,8 @@ def attention_plain(q, k, v, pos, scale, window, sinks, name):
     at most (dim + 8) 2^-24 times its sum of absolute products, in any order,
     and so is the running maximum that cancels; a weight, and the sum it is
     divided by, by twice that.  The fp32 sums of weights and of products add
-    (positions + 16) 2^-24.  The exponential is off by at most 2^-18.5 for fp16
-    and 2^-13.7 for bf16 (a polynomial of degree 4 or 3 on +-1/2 where it is not
-    the hardware's, 2^-21), in a weight and in the sum."""
+    (positions + 16) 2^-24.  The hardware's exponential is off by at most 2^-21,
+    in a weight and in the sum."""
     q, k, v = q.double(), k.double(), v.double()
     g = q.shape[1] // k.shape[1]
     kk, vv = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
@@ -148,7 +147,7 @@ def attention_plain(q, k, v, pos, scale, window, sinks, name):
     h = half_step(name)
     d, n = q.shape[2], k.shape[0]
     rel = 2 * h + h * h + 4 * (d + 8) * 2.0 ** -24 * big + 2 * (n + 16) * 2.0 ** -24
-    rel = rel + 2 * (2.0 ** -18.5 if name == "f16" else 2.0 ** -13.7)
+    rel = rel + 2 * 2.0 ** -21
     return out, rel * mass + 1e-30 + (2.0 ** -24 if name == "f16" else 0.0)  # fp16: half of its smallest number, rounded up
 
 
