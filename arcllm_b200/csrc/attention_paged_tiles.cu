@@ -582,7 +582,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
                 uint64_t sum[2] = {0ull, 0ull};
-                constexpr uint32_t kAtOnce = kTile == 80u ? 80u : 32u;  // columns between two stores
+                // columns between two stores: beside 96 scores a thread's registers hold the weights of 32
+                constexpr uint32_t kAtOnce = kTile == 80u ? 80u : 32u;
 #pragma unroll
                 for (uint32_t c0 = 0; c0 < kTile; c0 += kAtOnce) {
                     uint32_t pk[kAtOnce / 2u];
