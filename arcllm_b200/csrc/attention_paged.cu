@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1)
 #pragma unroll
                 for (int nt = 0; nt < D / 8; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
             }
-            if (!quick_wait(&bars[warp][s_cons], parity, err)) {
+            if (!warp_wait(&bars[warp][s_cons], parity, err, [] { return false; })) {
                 ok = false;
                 break;
             }

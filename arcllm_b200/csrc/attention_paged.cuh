@@ -81,12 +81,25 @@ struct Record {
     uint32_t valid, last_cta, row0, rows, kvh, pad[3];
 };
 
-// mbar_wait whose first tries do not read the global timer: the read takes longer
-// than most of these waits do, and what arrives meanwhile is seen after it.
-__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, unsigned int* err) {
-    for (int i = 0; i < 64; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait(bar, parity, err);
+// A wait of a whole warp, false once it has taken limit_ns (then with the timeout
+// bit) or `stop()` says so.  One vote decides for all lanes, so they go on or give
+// up together: what follows are instructions of the whole warp, which lanes that
+// decided for themselves at the end of the limit would not reach together.  The first
+// tries do not read the global timer: that takes longer than most of these waits do,
+// and what arrives meanwhile is seen after it.
+template <typename Stop>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int* err, Stop stop,
+                                          unsigned long long limit_ns = kWaitLimitNs) {
+    unsigned long long t0 = 0;
+    for (uint32_t n = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++n) {
+        if (n < 64u) continue;
+        const unsigned long long t = globaltimer();
+        if (n == 64u) t0 = t;
+        const bool late = t - t0 > limit_ns;
+        if (late) raise_error(err, ARC_DEV_ERR_TIMEOUT);
+        if (__any_sync(0xffffffffu, late || stop())) return false;
+    }
+    return true;
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -134,20 +134,11 @@ __device__ __forceinline__ uint32_t item_units(const Args& a, const Req& q, uint
     return kItemCost + span_of<T>(a, q.p0 + first, q.p0 + first + rows - 1u).n;
 }
 
-// A role's wait: false once any role has given up.  One vote decides for the
-// warp: a wait that is over costs 96 clocks this way, 215 with a branch of its
-// own for each lane (and the MMA warp waits six times per tile).
+// A role's wait: false once any role has given up.  One vote for the warp also is
+// the faster form: a wait that is over costs 96 clocks this way, 215 with a branch
+// of its own for each lane (and the MMA warp waits six times per tile).
 __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-    unsigned long long t0 = 0;
-    for (uint32_t n = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++n) {
-        if (n < 64u) continue;  // the first tries do not read the timer
-        const unsigned long long t = globaltimer();
-        if (n == 64u) t0 = t;
-        const bool late = t - t0 > kWaitLimitNs;
-        if (late) raise_error(err, ARC_DEV_ERR_TIMEOUT);
-        if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
-    }
-    return true;
+    return warp_wait(bar, parity, err, [&] { return *abort_flag != 0; });
 }
 
 // The 4 x 4 blocks of 16 bytes of four neighbouring lanes, transposed: v[k] of lane j becomes v[j] of lane k.
