@@ -371,11 +371,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++stage == L::kStages) stage = 0, phase ^= 1u;
             }
         }
-        if (!ok) {  // no copy may still be landing at the end
-            abort_flag = 1;
-            for (uint32_t k = issued > L::kStages ? issued - L::kStages : 0u; k < issued; ++k)
-                mbar_wait(&kv_full[k % L::kStages], (k / L::kStages) & 1u, err);
-        }
+        if (!ok) abort_flag = 1;
+        // No copy may still be landing at the end.  That is also waited for when all were issued: another role may have
+        // given up before it used the last ones (otherwise this is over long before the output is).
+        for (uint32_t k = issued > L::kStages ? issued - L::kStages : 0u; k < issued; ++k)
+            warp_wait(&kv_full[k % L::kStages], (k / L::kStages) & 1u, err, [] { return false; });
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) raise_error(err, ARC_DEV_ERR_BOUNDS);
       } else if (warp < 11) {
         // ---------------- MMA of half s ----------------
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) abort_flag = 1;
         mma_commit(&done, leader);
         __syncwarp();
-        mbar_wait(&done, 0, err);  // nothing of this CTA runs on the tensor core any more
+        warp_wait(&done, 0, err, [] { return false; });  // nothing of this CTA runs on the tensor core any more
       } else {
         // ---------------- TMA: queries ----------------
         uint32_t n[2] = {0, 0};
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) abort_flag = 1;
 #pragma unroll
         for (uint32_t s = 0; s < 2u; ++s)  // no copy may still be landing at the end
-            if (n[s] != 0u) mbar_wait(&q_full[s], (n[s] - 1u) & 1u, err);
+            if (n[s] != 0u) warp_wait(&q_full[s], (n[s] - 1u) & 1u, err, [] { return false; });
       }
     } else {
       if (any) {
