@@ -97,6 +97,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
     return true;
 }
 
+// The same where other CTAs of the cluster complete the phase with their stores:
+// an acquire at cluster scope, without which reads of what they stored are not
+// ordered behind the wait.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, unsigned int* err) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait_cluster(bar, parity)) {
+        if (globaltimer() - t0 > kWaitLimitNs) {
+            raise_error(err, ARC_DEV_ERR_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+
 // L2 policy for weight streams: every weight byte is read once per token, so
 // let it leave L2 first and keep activations / KV resident.
 __device__ __forceinline__ uint64_t l2_evict_first_policy() {

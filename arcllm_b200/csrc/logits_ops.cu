@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
         if (tid == 0 && blockIdx.x != 0)
             st_async_u64(shared_of(&s_keys[blockIdx.x], 0), key, shared_of(&keys_in, 0));
         if (tid == 0 && blockIdx.x == 0) {
-            if (gridDim.x > 1u && mbar_wait(&keys_in, 0, err))
+            if (gridDim.x > 1u && mbar_wait_cluster(&keys_in, 0, err))
                 for (uint32_t c = 1; c < gridDim.x; ++c) key = s_keys[c] > key ? s_keys[c] : key;
             p.best[row] = key ? (int32_t)~(uint32_t)(key & 0xffffffffull) : -1;
         }
