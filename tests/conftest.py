@@ -16,3 +16,14 @@ def pytest_configure(config):
 @pytest.fixture(scope="session")
 def golden():
     return np.load(os.path.join(ROOT, "tests", "golden", "reference_golden.npz"))
+
+
+# Their arguments are made-up addresses, and some calls pass all checks: they must fail for want of a device.
+MADE_UP_ADDRESSES = ("test_paged_cpu", "test_paged_refusals_cpu")
+
+
+def pytest_runtest_setup(item):
+    if item.module.__name__ in MADE_UP_ADDRESSES:
+        import torch
+        if torch.cuda.is_available():
+            pytest.skip("made-up addresses: only where there is no GPU")
