@@ -333,6 +333,37 @@ bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
     return x < y + nb && y < x + na;
 }
 
+// One level of the places of a cache's elements: n steps of `stride` elements.
+struct Level {
+    uint64_t n, stride;
+};
+
+// Page, token and head levels (those of one step left out), widest first; how many, or -1 where they do not
+// nest: where a step is shorter than all that the levels within it span, two places can be one.
+int cache_levels(const arcllm_cuda_paged_kv& kv, Level (&lv)[3]) {
+    const Level all[3] = {{kv.n_pages, kv.page_stride}, {kv.page_size, kv.token_stride}, {kv.kv_heads, kv.head_stride}};
+    int n = 0;
+    for (const Level& l : all)
+        if (l.n > 1u) lv[n++] = l;
+    std::sort(lv, lv + n, [](const Level& x, const Level& y) { return x.stride > y.stride; });
+    unsigned __int128 extent = kv.head_dim;
+    for (int i = n - 1; i >= 0; --i) {
+        if (lv[i].stride < extent) return -1;
+        extent += (unsigned __int128)lv[i].stride * (lv[i].n - 1u);
+    }
+    return n;
+}
+
+// Whether an element at sum of i * stride + dim, with i and dim in range, can equal one of another cache of the same
+// levels that begins `off` elements after it: with nested levels the difference of i is one of two at each level.
+bool caches_meet(const Level* lv, int n, __int128 off, uint32_t dim) {
+    if (n == 0) return off < (__int128)dim && -off < (__int128)dim;
+    const __int128 s = lv->stride, lo = off >= 0 ? off / s : -((-off + s - 1) / s), last = (__int128)lv->n - 1;
+    for (__int128 d = lo; d <= lo + 1; ++d)
+        if (d <= last && -d <= last && caches_meet(lv + 1, n - 1, off - d * s, dim)) return true;
+    return false;
+}
+
 }  // namespace
 
 int paged_plan(const PagedPlan& p, cudaStream_t stream) {
@@ -442,6 +473,15 @@ int rope_kv_paged(int act_type, const RopePaged& p, const arcllm_cuda_paged_kv& 
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: q_out overlaps q without being the same rows");
     if (meets_out(p.k, p.k_stride, kn) || meets_out(p.v, p.v_stride, kn))
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: q_out overlaps k or v");
+    // Two threads would write one element (attention, which only reads, takes such a cache).
+    Level lv[3];
+    const int levels = cache_levels(kv, lv);
+    if (levels < 0)
+        return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: strides that lay places of the cache over one another");
+    const int64_t between =
+        (int64_t)(reinterpret_cast<uintptr_t>(kv.v_pages) - reinterpret_cast<uintptr_t>(kv.k_pages));
+    if (caches_meet(lv, levels, between / 2, kv.head_dim))
+        return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: K and V of the cache share places");
     // 16-byte vectors where every vector starts on 16 bytes and no unit is part rotated (8192 rows of 32 / 8 heads 43 us);
     // else element by element (131 us)
     const bool vec = p.rot_dim % 16u == 0u && kv.head_dim % 16u == 0u && aligned16(p.q) && aligned16(p.k) &&

@@ -397,7 +397,10 @@ ARCLLM_CUDA_API int arcllm_cuda_argmax(const float *logits, uint32_t n, void *sc
 
 /* One layer's cache.  Element (page, token, head, dim) of K and of V lies at
  * page * page_stride + token * token_stride + head * head_stride + dim
- * (elements), so pages may be stored token by token or head by head. */
+ * (elements), so pages may be stored token by token or head by head.  What
+ * writes to a cache takes it only where no two places share an element: each
+ * stride at least what lies within its step, in whatever order the strides
+ * stand, and K and V apart (they may take turns in one array). */
 typedef struct {
     void *k_pages, *v_pages;
     uint64_t page_stride;
