@@ -556,10 +556,11 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
     const uint64_t width = (uint64_t)p.q_heads * kv.head_dim;
     if (p.q_stride < width || p.out_stride < width)
         return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: a row stride shorter than the row");
-    auto off16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) != 0u; };
-    if (off16(p.q) || off16(p.out) || off16(kv.k_pages) || off16(kv.v_pages) || off16(p.workspace) ||
-        p.q_stride % 8u || p.out_stride % 8u || kv.page_stride % 8u || kv.token_stride % 8u || kv.head_stride % 8u)
+    if (any_off(16u, p.q, p.out, kv.k_pages, kv.v_pages, p.workspace) || p.q_stride % 8u || p.out_stride % 8u ||
+        kv.page_stride % 8u || kv.token_stride % 8u || kv.head_stride % 8u)
         return set_error(ARC_E_ALIGNMENT, "attention paged: pointers and strides of 16 bytes");
+    if (any_off(4u, p.block_table, p.row_start, p.kv_total))
+        return set_error(ARC_E_ALIGNMENT, "attention paged: arrays of 32-bit words");
     if (kv.kv_heads > 1u && kv.head_stride != kv.head_dim && kv.head_stride != (uint64_t)kv.page_size * kv.token_stride)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: heads side by side in a token, or one after another");
     if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31))

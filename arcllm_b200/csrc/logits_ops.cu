@@ -493,6 +493,9 @@ int logits_process(int type, const LogitsProcess& p, cudaStream_t stream) {
     const uint64_t size = type == ARC_GGML_F32 ? 4u : 2u;
     const uintptr_t a = reinterpret_cast<uintptr_t>(p.logits), b = reinterpret_cast<uintptr_t>(p.out);
     if ((a | b) % size) return set_error(ARC_E_ALIGNMENT, "logits: pointers aligned to their type");
+    if (any_off(4u, p.history, p.prompt_len, p.total_len, p.repetition, p.frequency, p.presence, p.bias_start, p.bias_ids,
+                p.bias_values, p.mask, p.best))
+        return set_error(ARC_E_ALIGNMENT, "logits: arrays of 32-bit words");
     // in place (the same rows) or apart
     const uint64_t na = ((uint64_t)(p.n_rows - 1u) * p.stride + p.vocab) * size;
     const uint64_t nb = ((uint64_t)(p.n_rows - 1u) * p.out_stride + p.vocab) * size;

@@ -370,6 +370,9 @@ int paged_plan(const PagedPlan& p, cudaStream_t stream) {
     if (!p.kv_len || !p.new_len || !p.free_pages || !p.n_free || !p.block_table || !p.row_start || !p.kv_total ||
         !p.positions || !p.slots || !p.n_free_out)
         return set_error(ARC_E_INVALID_ARGUMENT, "paged plan: null pointer");
+    if (any_off(4u, p.kv_len, p.new_len, p.free_pages, p.n_free, p.block_table, p.row_start, p.kv_total, p.positions,
+                p.slots, p.n_free_out))
+        return set_error(ARC_E_ALIGNMENT, "paged plan: arrays of 32-bit words");
     if (p.n_requests == 0 || p.page_size == 0 || p.n_pages == 0 || p.table_stride == 0 || p.max_rows == 0 ||
         p.max_rows > 0x7fffffffu)
         return set_error(ARC_E_INVALID_ARGUMENT, "paged plan: zero size, or rows past 2^31");
@@ -465,6 +468,9 @@ int rope_kv_paged(int act_type, const RopePaged& p, const arcllm_cuda_paged_kv& 
     if (p.q_stride < qn || p.out_stride < qn || p.k_stride < kn || p.v_stride < kn)
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: a row stride shorter than the row");
     const uint64_t as = act_type == ARC_GGML_F32 ? 4u : 2u;
+    if (any_off(as, p.q, p.k, p.v) || any_off(2u, p.q_out, kv.k_pages, kv.v_pages) ||
+        any_off(4u, p.bq, p.bk, p.bv, p.positions, p.slots) || any_off(8u, p.freqs))
+        return set_error(ARC_E_ALIGNMENT, "rope paged: pointers aligned to their type");
     // in place (the same rows of the same type) or apart
     auto meets_out = [&](const void* x, uint64_t stride, uint64_t width) {
         return rows_meet(x, stride * as, width * as, p.q_out, p.out_stride * 2u, qn * 2u, p.rows);

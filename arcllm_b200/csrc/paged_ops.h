@@ -69,6 +69,12 @@ struct LogitsProcess {
 };
 int logits_process(int type, const LogitsProcess& p, cudaStream_t stream);
 
+// Whether any of the pointers is not on a multiple of n bytes (null is): an array's words have to be.
+template <typename... Ptr>
+bool any_off(uintptr_t n, const Ptr*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (n - 1u)) != 0u;
+}
+
 // Whether two arrays of rows share a byte (strides and widths in bytes).  Rows of one stride may lie side by side
 // in one array (parts of a fused projection); with different strides any overlap of the whole ranges counts.
 inline bool rows_meet(const void* a, uint64_t a_stride, uint64_t a_width, const void* b, uint64_t b_stride,

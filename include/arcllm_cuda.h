@@ -392,7 +392,8 @@ ARCLLM_CUDA_API int arcllm_cuda_argmax(const float *logits, uint32_t n, void *sc
  * arcllm_cuda_rope_kv_paged and arcllm_cuda_attention_paged run per layer,
  * arcllm_cuda_logits_process follows the LM head.  Nothing here allocates,
  * synchronises or reads back: lengths stay on the device and a captured step
- * replays with new ones.  Index arrays are int32.  Lengths or page numbers
+ * replays with new ones.  Index arrays are int32, and every array begins on a
+ * multiple of its type's size (ARC_E_ALIGNMENT otherwise).  Lengths or page numbers
  * that no step can have set the device error word's bounds bit (bit 1). */
 
 /* One layer's cache.  Element (page, token, head, dim) of K and of V lies at

@@ -57,3 +57,27 @@ def test_store_into_small_caches_of_every_kind():
         assert refused == (twice or not nested), (pages, page, heads, strides, off)
         seen.add((twice, nested))
     assert len(seen) == 4
+
+
+def test_arrays_that_are_not_aligned_to_their_type():
+    """(entry point, a call that passes, {argument: size of a word})"""
+    plan = [a[0], a[1], 8, 16, 100, a[2], a[3], a[4], 10, 64, a[5], a[6], a[7], a[8], a[9], None]
+    attn = [a[0], 512, kv(), a[1], 9, a[2], a[3], 5, 20, 3, 4, 0.1, 0, 0, a[4], 512, a[5], 1 << 30, None]
+    logits = [A.GGML_F16, a[0], 100, 2, 100, a[1], 7, a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], 4, a[11],
+              100, a[12], None]
+    biased = changed(changed(changed(ROPE, 7, a[7]), 8, a[8]), 9, a[9])
+    half = changed(ROPE, 0, A.GGML_BF16)
+    for f, good, words in (("paged_plan", plan, dict.fromkeys((0, 1, 5, 6, 7, 10, 11, 12, 13, 14), 4)),
+                           ("rope_kv_paged", biased, {1: 4, 3: 4, 5: 4, 7: 4, 8: 4, 9: 4, 10: 8, 14: 4, 15: 4, 19: 2}),
+                           ("rope_kv_paged", half, {1: 2, 3: 2, 5: 2}),
+                           ("attention_paged", attn, {0: 16, 3: 4, 5: 4, 6: 4, 14: 16, 16: 16}),
+                           ("logits_process", logits, {1: 2, 17: 2, **dict.fromkeys((5, 7, 8, 9, 10, 11, 12, 13, 14,
+                                                                                     15, 19), 4)})):
+        for i, n in words.items():
+            for off in range(1, n):
+                got = status("arcllm_cuda_" + f, changed(good, i, P(good[i].value + off)))
+                assert got == ALIGN, (f, i, off, got)
+            got = status("arcllm_cuda_" + f, changed(good, i, P(good[i].value + n)))
+            assert got not in (ALIGN, INVALID), (f, i, got)
+    for k in (dict(k_pages=(1 << 20) + 1), dict(v_pages=(2 << 20) + 1)):
+        assert rope(**k) == ALIGN
