@@ -551,8 +551,9 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: at most 4096 requests");
     if (p.max_rows > 0x7fffffffu || p.table_stride == 0)
         return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: bad shape");
-    if (!(p.scale > 0.f) || !std::isfinite(p.scale))
-        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: scale must be positive");
+    const float scale_log2 = (float)((double)p.scale * 1.4426950408889634074);
+    if (!(p.scale > 0.f) || !std::isfinite(scale_log2))
+        return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: scale must be positive, and finite in units of log 2");
     const uint64_t width = (uint64_t)p.q_heads * kv.head_dim;
     if (p.q_stride < width || p.out_stride < width)
         return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: a row stride shorter than the row");
@@ -563,7 +564,8 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
         return set_error(ARC_E_ALIGNMENT, "attention paged: arrays of 32-bit words");
     if (kv.kv_heads > 1u && kv.head_stride != kv.head_dim && kv.head_stride != (uint64_t)kv.page_size * kv.token_stride)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: heads side by side in a token, or one after another");
-    if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31))
+    if (kv.page_stride >= (1ull << 39) || kv.token_stride >= (1u << 31) || p.q_stride >= (1ull << 39) ||
+        p.out_stride >= (1ull << 39))
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "attention paged: a stride past 2^40 bytes");
     if (rows_meet(p.q, 2u * p.q_stride, 2u * width, p.out, 2u * p.out_stride, 2u * width, p.max_rows))
         return set_error(ARC_E_INVALID_ARGUMENT, "attention paged: out overlaps q");
@@ -576,7 +578,7 @@ int attention_paged(const AttnPaged& p, const arcllm_cuda_paged_kv& kv, cudaStre
     a.row_start = p.row_start, a.kv_total = p.kv_total;
     a.n_requests = p.n_requests, a.max_rows = p.max_rows, a.max_new = p.max_new;
     a.kv_heads = kv.kv_heads, a.gq = gq, a.page_size = kv.page_size, a.n_pages = kv.n_pages;
-    a.scale_log2 = (float)((double)p.scale * 1.4426950408889634074);
+    a.scale_log2 = scale_log2;
     a.window = std::min(p.window, 0x7fffffffu);  // positions are below 2^31: sums stay within 32 bits
     a.sinks = p.window ? std::min(p.sinks, 0x7fffffffu) : 0u;
     const bool bf = kv.type == ARC_GGML_BF16;

@@ -482,7 +482,7 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  *   block_table  as arcllm_cuda_paged_plan leaves it; entries of pages that no
  *                row sees (before the window) are not read as pages' numbers;
  *   max_new      at least the largest number of rows of one request;
- *   scale        on q.k, > 0 (1/sqrt(head_dim) unless the model says otherwise);
+ *   scale        on q.k, > 0 and at most 2.3e38 (1/sqrt(head_dim) unless the model says otherwise);
  *   workspace    arcllm_cuda_attention_paged_workspace bytes, any content;
  *                calls that may overlap in time need one each.
  * head_dim 64 or 128, q_heads/kv_heads 1..128, page_size a multiple of 16,

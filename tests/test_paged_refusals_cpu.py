@@ -81,3 +81,14 @@ def test_arrays_that_are_not_aligned_to_their_type():
             assert got not in (ALIGN, INVALID), (f, i, got)
     for k in (dict(k_pages=(1 << 20) + 1), dict(v_pages=(2 << 20) + 1)):
         assert rope(**k) == ALIGN
+
+
+def test_attention_strides_and_scales_past_what_its_arithmetic_holds():
+    """No tensor map steps 2^40 bytes; a scale whose multiple of log2 e is infinite has no scores."""
+    f = "arcllm_cuda_attention_paged"
+    good = [a[0], 512, kv(), a[1], 9, a[2], a[3], 5, 20, 30, 4, 0.1, 0, 0, a[4], 512, a[5], 1 << 30, None]
+    for i in (1, 15):
+        assert status(f, changed(good, i, 2 ** 39)) == SHAPE
+        assert status(f, changed(good, i, 2 ** 62)) == SHAPE
+    assert status(f, changed(good, 11, 2.5e38)) == INVALID
+    assert status(f, changed(good, 11, 2.3e38)) not in (INVALID, SHAPE)
