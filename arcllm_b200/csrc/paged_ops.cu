@@ -380,14 +380,18 @@ int paged_plan(const PagedPlan& p, cudaStream_t stream) {
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "paged plan: more than 2^31 - 1 slots");
     if (p.n_requests > kPlanMaxRequests)
         return set_error(ARC_E_UNSUPPORTED_SHAPE, "paged plan: at most 8192 requests");
-    // every CTA reads the inputs while the first one writes these
-    const uint64_t n4 = 4ull * p.n_requests;
-    const void* outs[] = {p.row_start, p.kv_total, p.positions, p.slots, p.n_free_out};
-    const uint64_t bytes[] = {n4 + 4u, n4, 4ull * p.max_rows, 4ull * p.max_rows, 4u};
-    for (int i = 0; i < 5; ++i)
-        if (overlap(outs[i], bytes[i], p.kv_len, n4) || overlap(outs[i], bytes[i], p.new_len, n4) ||
-            overlap(outs[i], bytes[i], p.n_free, 4u))
-            return set_error(ARC_E_INVALID_ARGUMENT, "paged plan: an output overlaps an input");
+    // every CTA reads the inputs and old table entries while others write, and each output is written by itself (how
+    // long the free list is only the device knows)
+    const uint64_t n4 = 4ull * p.n_requests, m4 = 4ull * p.max_rows;
+    const struct {
+        const void* at;
+        uint64_t bytes;
+    } array[] = {{p.row_start, n4 + 4u}, {p.kv_total, n4}, {p.positions, m4}, {p.slots, m4}, {p.n_free_out, 4u},
+                 {p.block_table, n4 * p.table_stride}, {p.kv_len, n4}, {p.new_len, n4}, {p.n_free, 4u}};
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 9; ++j)
+            if (overlap(array[i].at, array[i].bytes, array[j].at, array[j].bytes))
+                return set_error(ARC_E_INVALID_ARGUMENT, "paged plan: an output overlaps another array");
     const uint32_t smem = 12u * p.n_requests;
     if (smem > 48u * 1024u - 1024u) {
         const cudaError_t e = allow_shared<paged_plan_kernel>(12 * kPlanMaxRequests);

@@ -426,7 +426,8 @@ typedef struct {
  * a table row too short, a negative length) sets the bounds bit and lays out
  * an empty step instead: row_start all 0, kv_total = kv_len, slots -1, nothing
  * taken.  A row whose page number is outside [0, n_pages) gets slot -1 and
- * sets the bounds bit.  Outputs may not overlap kv_len, new_len or n_free. */
+ * sets the bounds bit.  No output (block_table is one) overlaps another
+ * array of the call. */
 ARCLLM_CUDA_API int arcllm_cuda_paged_plan(const int32_t *kv_len, const int32_t *new_len, uint32_t n_requests,
                                            uint32_t page_size, uint32_t n_pages, const int32_t *free_pages,
                                            const int32_t *n_free, int32_t *block_table, uint32_t table_stride,

@@ -92,3 +92,18 @@ def test_attention_strides_and_scales_past_what_its_arithmetic_holds():
         assert status(f, changed(good, i, 2 ** 62)) == SHAPE
     assert status(f, changed(good, 11, 2.5e38)) == INVALID
     assert status(f, changed(good, 11, 2.3e38)) not in (INVALID, SHAPE)
+
+
+def test_plan_into_arrays_that_overlap():
+    """Outputs one over another, the table over an input or an output."""
+    f = "arcllm_cuda_paged_plan"
+    good = [a[0], a[1], 8, 16, 100, a[2], a[3], a[4], 10, 64, a[5], a[6], a[7], a[8], a[9], None]
+    size = {0: 32, 1: 32, 6: 4, 7: 320, 10: 36, 11: 32, 12: 256, 13: 256, 14: 4}
+    for i in (7, 10, 11, 12, 13, 14):
+        for j in size:
+            if i == j:
+                continue
+            for at in (good[j].value, good[j].value + size[j] - 4, good[j].value + 4 - size[i]):
+                assert status(f, changed(good, i, P(at))) == INVALID, (i, j, at)
+            for at in (good[j].value + size[j], good[j].value - size[i]):
+                assert status(f, changed(good, i, P(at))) != INVALID, (i, j, at)
