@@ -27,8 +27,9 @@ using namespace paged;
 // operand is a (row, head of the group) pair).  Parts of an item that lie in one
 // CTA are joined here, what CTAs share by the join kernel.
 // HBM bound: 64 requests of 1 row over up to 8192 positions, 8 heads of 128 (1.07
-// GB) 173 us with the join, 6.2 TB/s, 0.95 of the measured copy rate.  One request
-// over 1027 positions 10.5 us, of which the join's launch is 3.5.
+// GB) 177 us with the join, 6.1 TB/s, 0.93 of the measured copy rate, replayed in a
+// graph (180 to 194 us called from Python); 4 requests over up to 79508 positions (1.12
+// GB) 181 us.  One request over 1027 positions 11 us, a third of it the join's launch.
 constexpr uint32_t kRowWarps = 8, kRowTile = 16;
 
 struct Segment {  // an unfinished item of a warp

@@ -16,8 +16,8 @@ namespace paged {
 constexpr uint32_t kSms = 148;          // one CTA per SM in both attention kernels
 constexpr uint32_t kTileRows = 256;     // packed rows of an item of the tile kernel
 // Requests with at most so many packed rows go to the rows kernel, whose matrix operand has 16.  32 requests over
-// 4096 positions of 8 heads: 16 rows there 97 us (1 row 93), 17 rows in the tile kernel 119 us (32 rows 134); 64 over
-// 512: 40 and 53 us; 4 over 4096: 24 and 25 us.
+// 4096 positions of 8 heads: 16 rows there 97 us (4 rows 94), 17 rows in the tile kernel 117 to 121 us (32 rows 122); 64
+// over 512: 40 and 50 to 53 us; 4 over 4096: 23 and 24 to 26 us.
 constexpr uint32_t kRowMax = 16;
 constexpr uint32_t kMaxRequests = 4096; // unit offsets of the requests in shared memory
 

@@ -15,14 +15,13 @@
 //                     item before is there
 // Tensor memory (512 columns of 128 rows) decides the tile: with O in 2 x D of
 // them, S and P of both halves fit side by side for 80 positions at D = 128, so S
-// of the next tile is formed as soon as a softmax has S in its registers.  With
-// tiles of 128 P had to lie over S, S of the next tile had to wait for the
-// product, and the chain weights - products - S - softmax of one half set the
-// pace (3400 clocks for 128 positions, against 2290 for 80).  At D = 64 a tile is
-// 96 positions, what a thread's registers hold, and there is room for two P of
-// each half: P then needs no wait for the product before (12 requests, 16 heads,
-// window 1024: 105.2 -> 103.2 us).  Two P at D = 128 would leave tiles of 64
-// (12000 rows: 470 -> 504 us).
+// of the next tile is formed as soon as a softmax has S in its registers; over a
+// tile of 128, P has to lie over S, and S of the next tile waits for the product.
+// At D = 128 that is not shown to pay: 493 us for the 12000 rows below with tiles of
+// 128, 475 to 500 with 80.  At D = 64 a tile is 96 positions, what a thread's
+// registers hold, and there is room for two P of each half: P then needs no wait
+// for the product before (12 requests, 16 heads, window 1024: 105.2 -> 103.2 us).
+// Two P at D = 128 would leave tiles of 64 (12000 rows: 470 -> 504 us).
 // O is scaled only when a row's maximum has grown by more than 2^8 since the
 // last time (the sums carry the same factor, so the result is the same).
 // K and V tiles are built from boxes of positions that divide the page and the
@@ -30,13 +29,15 @@
 // All waits are bounded: on a timeout the roles leave their loops, drain what
 // they started and the error word is set.
 // Measured: 12000 new rows of 2 requests, 28 / 4 heads of 128, contexts of 2048
-// before them (0.50 TFLOP): 470 to 500 us, as the clock varies with the power,
-// so 1.0 to 1.07 PFLOP/s, 0.60 to 0.65 of the measured matrix rate.  The bound is
-// the softmax's chain per tile: 2290 clocks, of which the exponentials (16 per
-// clock and SM) are 1280 and both halves' products 1460 beside them; the rest is
-// issue and hand-over (a wait that is over costs 100 clocks, and the chain has
-// three).  Starting the halves half a tile apart changed nothing, nor did a quarter
-// of the exponentials as polynomials on the FMA units (0.4 %; half of them 3 % slower).
+// before them (0.50 TFLOP): 483 to 492 us one after another in a graph, 1.02 to 1.04
+// PFLOP/s, 0.62 of the measured matrix rate; called from Python with pauses between
+// 534 to 555 us, 0.55 to 0.57 (the clock follows the power).  The bound is the softmax's
+// chain: 2350 clocks per tile of 80 (2580 per tile of 96 at D = 64 with a window) and
+// 4700 per item, where the exponentials (16 per clock and SM) of both halves are 1280
+// and both halves' products 1460 beside them; the rest is issue and hand-over (a wait
+// that is over costs 100 clocks, and the chain has three).  Starting the halves half a
+// tile apart changed nothing, nor did a quarter of the exponentials as polynomials on
+// the FMA units (0.4 %; half of them 3 % slower).
 #include <algorithm>
 
 #include "arcllm_cuda_internal.h"

@@ -94,16 +94,18 @@ __device__ __forceinline__ uint32_t shared_of(const void* p, uint32_t rank) {  /
 // Rows need not start on 16 bytes: token t is numbered t + a, a the elements
 // between the last 16-byte boundary and the row's first, so that vectors of V
 // numbers are aligned (the first and the last may be partly outside the row).
-// Without Shift every row starts on 16 bytes and a is 0: what Shift needs costs 44
-// instead of 41 us for 128 rows of 152064 fp32 (single numbers, as where logits and
-// out lie differently to 16 bytes, 110 us).
-// 128 rows of 152064 fp32 with histories of 4096, biases and masks: 41 us, 3.9
+// Without Shift every row starts on 16 bytes and a is 0: what Shift needs costs 58
+// instead of 47 us for 128 rows of 152064 fp32 (single numbers, as where logits and
+// out lie differently to 16 bytes, 116 us).
+// 128 rows of 152064 fp32 with histories of 4096, biases and masks: 47 us, 3.4
 // TB/s, of which counting is about 8 us with little traffic; without constraints
-// 31 us, 5.0 TB/s.  A row by itself: 7.8 us, latency.  Forming the named tokens in
-// the stream took 56 us (a warp nearly always has one, and then all of it waits for
-// the division), a choice token by token 47, mask words loaded where they are used
-// 43; bulk copies into shared memory ahead of the stream, or each register loaded
-// again as soon as its vector is written, were slower than this.
+// 32 us, 4.9 TB/s.  fp16 and bf16: 35 and 36 us, without constraints 18 (4.4 TB/s).  A
+// row by itself with a history of 301: 8.4 us, latency.  With one set of inputs over and
+// over, part of it in L2, the first of these is 41 us; in that measure forming the named
+// tokens in the stream took 56 (a warp nearly always has one, and then all of it waits
+// for the division), a choice token by token 47, mask words loaded where they are used
+// 43; bulk copies into shared memory ahead of the stream, or each register loaded again
+// as soon as its vector is written, were slower than this.
 template <typename T, int V, bool Shift>
 __global__ void __launch_bounds__(kLogitsThreads, 2)
     logits_process_kernel(LogitsProcess p, uint32_t slice, uint32_t chunk, unsigned int* err) {
@@ -403,8 +405,8 @@ __global__ void __launch_bounds__(kLogitsThreads, 2)
 template <typename T, int V, bool Shift>
 cudaError_t launch_logits(const LogitsProcess& p, uint32_t row0, uint32_t rows, cudaStream_t stream) {
     // CTAs per row: as many as give the least waves x (tokens of a CTA + what a CTA costs beside them).  Measured for
-    // 152064 tokens with all constraints: 128 rows 73 / 48 / 53 / 69 us with 1 / 2 / 4 / 8, 64 rows 66 / 36 / 28 / 36, 20
-    // rows 62 / 34 / 23 / 20.
+    // 152064 tokens with all constraints: 128 rows 61 / 46 / 52 / 69 / 108 us with 1 / 2 / 4 / 8 / 16, 64 rows 54 / 32 / 28
+    // / 36 / 57, 20 rows 48 / 27 / 19 / 19 / 23, 1 row 46 / 26 / 19 / 15 / 13.
     constexpr uint64_t kSlots = 2u * 148u, kCtaCost = 7500u;
     uint32_t ctas = 1;
     uint64_t least = ~0ull;

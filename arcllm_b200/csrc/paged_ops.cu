@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t last_not_above(const int32_t* v, uint32_t n,
 // Every CTA scans all requests by itself (a few KB out of L2) and then fills
 // its share of the rows and of the new table entries, so one launch does it
 // without a grid-wide wait: the call is bounded by launch and load latency (256
-// requests of a token 3.4 us, 96 requests with 48 chunks of up to 1024 rows 5.1 us).
+// requests of a token 3.6 us, 96 requests with 48 chunks of up to 1024 rows 5.3 us).
 // total_r = kv_r + new_r; request r starts at row sum of new over the requests
 // before it and takes ceil(total_r / page) - ceil(kv_r / page) pages from the
 // end of the free list, after the requests before it.
@@ -207,9 +207,9 @@ __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
 // Angles pos * freq are formed and reduced to a fraction of a turn in 64 bits
 // (at 16384 an fp32 product is already 1e-3 off), then sin and cos in fp32.
 // Bounded by HBM traffic for many rows and by latency for few: 8192 rows of 32 / 8
-// heads of 128, bf16, 43 us (4.7 TB/s; 64 us with a row per CTA and none read
-// ahead, 48 with the unit worked out anew for each row), fp32 51 us (5.9 TB/s); 48
-// rows 3.1 us.  Two or three rows ahead, 3 or 4 CTAs' worth of threads per SM, or
+// heads of 128, bf16, 44 us (4.6 TB/s; 64 us with a row per CTA and none read
+// ahead, 48 with the unit worked out anew for each row), fp32 52 us (5.8 TB/s); 48
+// rows 3.3 us.  Two or three rows ahead, 3 or 4 CTAs' worth of threads per SM, or
 // units of 32 elements were 0 to 40 % slower, and without the angles it takes the same.
 constexpr uint32_t kRopeThreads = 512;
 template <typename TA, typename TC, int V>
@@ -492,8 +492,8 @@ int rope_kv_paged(int act_type, const RopePaged& p, const arcllm_cuda_paged_kv& 
         (int64_t)(reinterpret_cast<uintptr_t>(kv.v_pages) - reinterpret_cast<uintptr_t>(kv.k_pages));
     if (caches_meet(lv, levels, between / 2, kv.head_dim))
         return set_error(ARC_E_INVALID_ARGUMENT, "rope paged: K and V of the cache share places");
-    // 16-byte vectors where every vector starts on 16 bytes and no unit is part rotated (8192 rows of 32 / 8 heads 43 us);
-    // else element by element (131 us)
+    // 16-byte vectors where every vector starts on 16 bytes and no unit is part rotated (8192 rows of 32 / 8 heads 44 us);
+    // else element by element (132 us)
     const bool vec = p.rot_dim % 16u == 0u && kv.head_dim % 16u == 0u && aligned16(p.q) && aligned16(p.k) &&
                      aligned16(p.v) && aligned16(p.q_out) && aligned16(kv.k_pages) && aligned16(kv.v_pages) &&
                      ((p.q_stride | p.k_stride | p.v_stride) * as) % 16u == 0u && p.out_stride % 8u == 0u &&

@@ -425,7 +425,8 @@ typedef struct {
  * A step that does not fit (more than max_rows rows, more pages than are free,
  * a table row too short, a negative length) sets the bounds bit and lays out
  * an empty step instead: row_start all 0, kv_total = kv_len, slots -1, nothing
- * taken.  A row whose page number is outside [0, n_pages) gets slot -1 and
+ * taken.  (arcllm_cuda_attention_paged takes up to 4096 requests, and pages of a
+ * multiple of 16.)  A row whose page number is outside [0, n_pages) gets slot -1 and
  * sets the bounds bit.  No output (block_table is one) overlaps another
  * array of the call. */
 ARCLLM_CUDA_API int arcllm_cuda_paged_plan(const int32_t *kv_len, const int32_t *new_len, uint32_t n_requests,
@@ -459,9 +460,9 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_freqs(int scaling, uint32_t rot_dim, double
  *   freqs      rot_dim/2 doubles (device).
  * Angles are formed in 64 bits, so positions are not limited by a table.
  * q_out may be q itself (same type, same stride), and overlaps none of q, k, v
- * otherwise.  Slots must differ from one another (of rows with one slot, any one
- * may be stored).  16-byte aligned rows and rot_dim, head_dim % 16 == 0 take the
- * vector form. */
+ * otherwise.  Slots must differ from one another: one that several rows name is
+ * left with pieces of any of them.  16-byte aligned rows and rot_dim, head_dim %
+ * 16 == 0 take the vector form. */
 enum arcllm_rope_layout { ARC_ROPE_INTERLEAVED = 0, ARC_ROPE_HALVES = 1 };
 ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint64_t q_stride, const void *k,
                                               uint64_t k_stride, const void *v, uint64_t v_stride, const float *bq,
@@ -478,8 +479,9 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  * p = kv_total[r] - n + i, n its number of rows, and sees positions j <= p;
  * with window > 0 only those with j > p - window or j < sinks.
  *   q, out       [max_rows][q_heads*head_dim] of the cache's type, row strides
- *                in elements, apart from one another; rows of no request are
- *                left as they were;
+ *                in elements, apart from one another (and from the cache, the
+ *                index arrays and the workspace); rows of no request are left as
+ *                they were;
  *   block_table  as arcllm_cuda_paged_plan leaves it; entries of pages that no
  *                row sees (before the window) are not read as pages' numbers;
  *   max_new      at least the largest number of rows of one request;
@@ -490,9 +492,17 @@ ARCLLM_CUDA_API int arcllm_cuda_rope_kv_paged(int act_type, const void *q, uint6
  * n_requests <= 4096; pointers 16-byte aligned, strides multiples of 8; the
  * heads of a page side by side in each token (head_stride = head_dim) or one
  * after another (head_stride = page_size * token_stride).
+ * Scores, softmax statistics and sums are fp32.  q has the cache's 16 bits (the
+ * two operators above take fp32 q), so a score is off by up to half a step of q,
+ * and the weights of the second product are rounded to the cache's type, half a
+ * step of each, as the output is.
+ * A step captured with max_new as its capacity also launches the kernel for many
+ * rows when its lengths at replay are single tokens (3 to 5 us).
  * A request whose lengths do not fit (kv_total < n, n > max_new, a table row
  * too short, rows past max_rows) is skipped and sets the bounds bit; a page
- * number outside [0, n_pages) sets it too and reads as zeros.  What lies at
+ * number outside [0, n_pages) sets it too and reads as zeros; a step of more than
+ * 2^31 - 1 tiles of 16 positions (over all requests and KV heads) sets it and is
+ * skipped as a whole.  What lies at
  * positions that no row of a request sees may be anything; an infinite or NaN
  * value at a position that one of its rows sees may make others of its rows NaN
  * (a weight of 0 times it). */
