@@ -372,11 +372,13 @@ def _plain_attention(s):
 
 def _call_logits(s):
     c, m = s["c"], s["mask"]
+    b = [s[k] for k in ("bias_start", "bias_ids", "bias_values")]
+    if b[0] is not None and b[1].numel() == 0:  # no row has an entry: nothing to point at
+        b = [None] * 3
     _call("arcllm_cuda_logits_process", GGML[c["type"]], _ptr(s["logits"]), s["logits"].stride(0), c["rows"],
           c["vocab"], _ptr(s["history"]), s["history"].shape[1], _ptr(s["prompt_len"]), _ptr(s["total_len"]),
-          _ptr(s["repetition"]), _ptr(s["frequency"]), _ptr(s["presence"]), _ptr(s["bias_start"]),
-          _ptr(s["bias_ids"]), _ptr(s["bias_values"]), _ptr(m), 0 if m is None else m.shape[1], _ptr(s["out"]),
-          s["out"].stride(0), _ptr(s["best"]))
+          _ptr(s["repetition"]), _ptr(s["frequency"]), _ptr(s["presence"]), _ptr(b[0]), _ptr(b[1]), _ptr(b[2]),
+          _ptr(m), 0 if m is None else m.shape[1], _ptr(s["out"]), s["out"].stride(0), _ptr(s["best"]))
     return s["out"], s["best"]
 
 
