@@ -529,7 +529,8 @@ ARCLLM_CUDA_API int arcllm_cuda_attention_paged(const void *q, uint64_t q_stride
  *                (prompt_len null: none), [prompt_len, total_len) generated;
  *                values outside the vocabulary are passed over;
  *   repetition, frequency, presence  [n_rows], each nullable;
- *   bias_start   [n_rows + 1] into bias_ids and bias_values; null: none;
+ *   bias_start   [n_rows + 1] into bias_ids and bias_values, neither of them null,
+ *                whatever bias_start holds; null: none;
  *   mask         [n_rows][mask_stride] words, bit t % 32 of word t / 32 set:
  *                token t is allowed; null: all are;
  *   out          of the logits' type (F32, F16 or BF16), rounded to it; may be
